@@ -5,16 +5,19 @@ The compute lives in hand-written HIP kernels (``csrc/``) behind the C ABI of
 
 * ``backend.HipBackend`` -- ``attention`` / ``attention_fixed`` /
   ``attention_prefill`` / ``attention_ragged`` with the reference call
-  signatures (breezetoken/backends.py:47-51, 657-706; model/prefill.py:56-68);
+  signatures (breezetoken/backends.py:47-51, 657-706; model/prefill.py:56-68),
+  and a decode step over a paged cache: ``attn_prep_paged``, ``attention_paged``,
+  ``beam_select``, ``fork_pages``, ``compact_pages``;
 * ``kvcache.KVCache`` -- the fixed-capacity bf16 cache with the reference's
   ``(max_context, n_kv * head_dim)`` views (breezetoken/model/config.py:100-111);
+* ``kvcache.PagedKVCache`` -- many sequences' cache in shared pages;
 * ``workloads`` -- seeded synthetic inputs for the benchmark configurations;
 * ``build`` -- compiles ``libbreezetoken_amd.so`` for gfx950.
 """
 
-from .kvcache import KVCache
+from .kvcache import KVCache, PagedKVCache
 
-__all__ = ["KVCache", "HipBackend", "make_backend"]
+__all__ = ["KVCache", "PagedKVCache", "HipBackend", "make_backend"]
 __version__ = "0.1.0"
 
 

@@ -119,6 +119,34 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_vp, _vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _c_i64, _vp],
     ),
+    "bt_paged_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "bt_gqa_decode_paged": (
+        ctypes.c_int,
+        [_vp, _c_i32, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64, _c_i32, _vp,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _vp, _c_i64, _vp, _c_i32, _c_i64, _vp],
+    ),
+    "bt_attn_prep_paged": (
+        ctypes.c_int,
+        [_vp, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _vp, _c_f32, _vp, _vp, _c_i32,
+         _c_i32, _c_i32, _vp, _vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64,
+         _c_i32, _c_i32, _vp],
+    ),
+    "bt_pages_workspace_bytes": (_c_i64, [_c_i32, _c_i32]),
+    "bt_fork_pages": (
+        ctypes.c_int,
+        [_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _vp, _c_i32, _c_i32, _vp, _vp, _c_i32, _vp,
+         _c_i32, _vp, _vp, _vp, _vp, _c_i64, _vp],
+    ),
+    "bt_compact_pages": (
+        ctypes.c_int,
+        [_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _vp, _c_i32, _c_i32, _vp, _c_i32, _vp, _vp,
+         _vp, _vp, _c_i64, _vp],
+    ),
+    "bt_beam_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32]),
+    "bt_beam_select": (
+        ctypes.c_int,
+        [_vp, _c_i32, _c_i64, _c_i64, _vp, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _c_i64, _vp],
+    ),
 }
 
 _lock = threading.Lock()

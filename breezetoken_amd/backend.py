@@ -26,7 +26,14 @@ and adds the operators the reference runs outside the protocol:
 * ``gdn_decode(q, k, v, g, beta, state, scale, eps)``: the Gated DeltaNet
   one-token step with the f32 state updated in place (backends.py:79-92);
 * ``linear(x, w)``: the decode matvec x (K,) f32 . w (K, N) bf16 -> (N,) f32
-  of every projection and the vocabulary head (backends.py:36-37).
+  of every projection and the vocabulary head (backends.py:36-37);
+* over a paged cache (``kvcache.PagedKVCache``), for many sequences at once:
+  ``attn_prep_paged(...)``: the preparation of any number of tokens, rotary
+  positions in either layout; ``attention_paged(q, k, v, table, lens, scale)``:
+  one new token per sequence; ``fork_pages(...)`` and ``compact_pages(...)``:
+  sequences that continue others, room for their next tokens, pages moved
+  together; ``beam_select(logits, scores, beams)``: beam search's selection,
+  whose parents ``fork_pages`` takes.
 
 Every launch goes through libbreezetoken_amd.so on torch's current stream with
 no host synchronisation, so the calls can be captured in a hipGraph
@@ -39,6 +46,7 @@ backends.py:698 with graph.py:127-133).
 from __future__ import annotations
 
 import ctypes
+import math
 import operator
 from collections import OrderedDict
 
@@ -46,11 +54,13 @@ import torch
 
 from . import _lib
 from ._lib import BT_DTYPE_BF16, BT_DTYPE_F32, check
+from .kvcache import PAGE_SIZES
 
 SERVED_HEAD_DIMS = (64, 128, 256)
 SERVED_PREP_DIMS = (64, 128, 256, 512)
 SERVED_PREFILL_HEAD_DIMS = (128, 256)
 MAX_GROUP = 8
+MAX_BEAMS = 64
 
 
 def rope_tables(cap: int, rope_dim: int, theta: float, device: str | torch.device = "cuda"):
@@ -62,6 +72,45 @@ def rope_tables(cap: int, rope_dim: int, theta: float, device: str | torch.devic
     phases = torch.outer(torch.arange(cap, device=device, dtype=torch.float32), inv)
     freqs = torch.cat((phases, phases), dim=-1)
     return freqs.cos(), freqs.sin()
+
+
+def rope_tables_scaled(cap: int, rope_dim: int, theta: float, method: str, factor: float, trained: int | None = None,
+                       device: str | torch.device = "cuda"):
+    """cos/sin (cap, rope_dim) f32 tables for contexts ``factor`` times as long as
+    the ``trained`` one, both halves equal.  Angles are taken in 64 bits: at
+    position 10^6 an f32 angle is off by up to 0.03.  ``method``:
+
+    * ``linear``: positions divided by the factor;
+    * ``ntk``: theta * factor^(rope_dim / (rope_dim - 2)), so that the slowest pair
+      is slowed by the factor and the fastest keeps its rate;
+    * ``yarn`` (Peng et al., 2023): pairs that turn at least 32 times over the
+      trained context keep their rate, those that turn at most once are slowed by
+      the factor, a linear ramp between; the tables carry 0.1 ln(factor) + 1."""
+    if rope_dim < 2 or rope_dim % 2 or cap < 1:
+        raise ValueError(f"invalid rope_dim {rope_dim} or cap {cap}")
+    if not factor >= 1.0 or not theta > 1.0:
+        raise ValueError("factor must be at least 1, theta above 1")
+    half, attn = rope_dim // 2, 1.0
+    i = torch.arange(half, dtype=torch.float64)
+    inv = theta ** (-i / half)
+    if method == "linear":
+        inv = inv / factor
+    elif method == "ntk":
+        if rope_dim > 2:
+            inv = (theta * factor ** (rope_dim / (rope_dim - 2))) ** (-i / half)
+    elif method == "yarn":
+        if not trained or trained < 1:
+            raise ValueError("yarn needs the trained context length")
+        low, high = (half * math.log(trained / (2 * math.pi * turns)) / math.log(theta) for turns in (32, 1))
+        low, high = max(0, math.floor(low)), min(half - 1, math.ceil(high))
+        slow = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv / factor * slow + inv * (1 - slow)
+        attn = 0.1 * math.log(factor) + 1.0
+    else:
+        raise ValueError(f"unknown method {method!r}")
+    phases = torch.outer(torch.arange(cap, device=device, dtype=torch.float64), inv.to(device))
+    freqs = torch.cat((phases, phases), dim=-1)
+    return (freqs.cos() * attn).float(), (freqs.sin() * attn).float()
 
 
 def decode_unserved(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, device: torch.device | None = None) -> str | None:
@@ -776,6 +825,269 @@ class HipBackend:
         )
         check("bt_gdn_decode", rc)
         return out
+
+    # ------------------------------------------------------------ paged caches
+    # Workspaces here are allocated by each call on its stream, from torch's
+    # allocator: calls on two streams, or two captured graphs, share none.
+    def _run(self, name: str, *args) -> None:
+        """Launch on this backend's device, whichever is current."""
+        fn, dev = getattr(self._lib, name), self._dev
+        if torch.cuda.current_device() == dev.index:
+            rc = fn(*args, _stream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, _stream(dev))
+        if rc:
+            check(name, rc)
+
+    def _on_device(self, **tensors: torch.Tensor | None) -> None:
+        for name, t in tensors.items():
+            if t is not None and t.device != self._dev:
+                raise RuntimeError(f"{name} must live on the backend's device")
+
+    @staticmethod
+    def _check_ints(name: str, t: torch.Tensor, n: int) -> None:
+        if t.dtype is not torch.int32 or t.ndim != 1 or t.shape[0] != n or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} values")
+
+    @staticmethod
+    def _check_table(table: torch.Tensor) -> None:
+        if table.dtype is not torch.int32 or table.ndim != 2 or not table.is_contiguous() or table.shape[1] < 1:
+            raise RuntimeError("table must be a contiguous int32 (rows, pages) tensor")
+
+    def _paged_kv(self, k: torch.Tensor, v: torch.Tensor, dim: int) -> tuple[int, int, int, int, int, int]:
+        """Pages, page size, kv heads and the strides of a page, token and head."""
+        if k.ndim != 4 or v.shape != k.shape:
+            raise RuntimeError("k/v must be (pages, page_size, Hkv, D) with equal shapes")
+        pages, size, groups, kdim = k.shape
+        if kdim != dim or groups < 1 or pages < 1:
+            raise RuntimeError(f"a cache {tuple(k.shape)} does not hold heads of {dim}")
+        if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
+            raise RuntimeError("the MI355X path serves a bf16 KV cache only")
+        if size not in PAGE_SIZES:
+            raise RuntimeError(f"page size {size} is not served {PAGE_SIZES}")
+        sp, st, sh, sd = k.stride()
+        if sd != 1 or v.stride() != k.stride():
+            raise RuntimeError("k/v need unit d-stride and identical strides")
+        # The stride of a dimension of one is whatever its maker left there.
+        return pages, size, groups, sp if pages > 1 else size * groups * dim, st, sh if groups > 1 else dim
+
+    def attention_paged(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                        lens: torch.Tensor, scale: float, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Decode attention of one new token per sequence over a paged cache.
+
+        q (B, H, D) f32 or bf16; k/v (pages, page_size, Hkv, D) bf16, any strides
+        with unit d-stride; table (B, P) int32 page ids; lens (B,) int32 valid
+        tokens, the new one among them -> (B, H, D) in ``out_dtype``.  Everything is
+        read on the device; a row without tokens gives zeros, a table entry outside
+        the cache holds no keys."""
+        if q.ndim != 3:
+            raise RuntimeError("paged attention expects q (B, H, D)")
+        batch, heads, dim = q.shape
+        pages, size, groups, sp, st, sh = self._paged_kv(k, v, dim)
+        if heads < 1 or heads % groups:
+            raise RuntimeError(f"q heads {heads} / kv heads {groups} do not form a GQA group")
+        if dim not in SERVED_HEAD_DIMS or heads // groups > MAX_GROUP:
+            raise RuntimeError(f"shape H={heads} Hkv={groups} D={dim} is not served")
+        self._check_table(table)
+        if table.shape[0] != batch:
+            raise RuntimeError("table needs one row per sequence")
+        self._check_ints("lens", lens, batch)
+        self._on_device(q=q, k=k, v=v, table=table, lens=lens)
+        q_code, out_code = _dtype_code(q.dtype), _dtype_code(out_dtype)
+        out = torch.empty((batch, heads, dim), dtype=out_dtype, device=self._dev)
+        if batch == 0:
+            return out
+        q = q.contiguous()
+        per_seq = table.shape[1]
+        nbytes = self._lib.bt_paged_workspace_bytes(batch, heads, groups, dim, min(per_seq * size, 0x7FFFFFFF))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev) if nbytes else None
+        self._run("bt_gqa_decode_paged", q.data_ptr(), q_code, heads * dim, k.data_ptr(), v.data_ptr(), sp, st, sh, pages,
+                  size, table.data_ptr(), per_seq, per_seq, lens.data_ptr(), batch, heads, groups, dim, float(scale),
+                  _ptr(ws), nbytes, out.data_ptr(), out_code, heads * dim)
+        return out
+
+    def attn_prep_paged(
+        self, qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor | None, eps: float,
+        cos: torch.Tensor | None, sin: torch.Tensor | None, pos: torch.Tensor, rope_dim: int, k: torch.Tensor,
+        v: torch.Tensor, table: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+        rows: torch.Tensor | None = None, gated: bool = True, interleaved: bool = False,
+        q_dtype: torch.dtype = torch.float32,
+    ) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """``attn_prep`` for any number of tokens over a paged cache, in one launch.
+
+        qkv (T, row) f32 or bf16: [H x (q | gate) | Hkv x k | Hkv x v], or with
+        ``gated=False`` [H x q | Hkv x k | Hkv x v].  q and k are normalised
+        (q_norm/k_norm f32, or None), their first ``rope_dim`` values rotated by
+        table row pos[t] (cos/sin of ``rope_tables`` or ``rope_tables_scaled``, or
+        None): halves against each other, or neighbours where ``interleaved``.  k and
+        v go to token pos[t] of table row rows[t] (default: row t), rounded to bf16;
+        a token without a slot there writes none, and two tokens of a call must not
+        name one slot.  pos and rows (T,) int32.  Returns q (T, H, D) in ``q_dtype``
+        and the gate as a (T, H, D) view of ``qkv`` (None without one)."""
+        D, heads, kv_heads = int(head_dim), int(heads), int(kv_heads)
+        if D not in SERVED_PREP_DIMS:
+            raise RuntimeError(f"head_dim {D} is not served {SERVED_PREP_DIMS}")
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise RuntimeError(f"q heads {heads} / kv heads {kv_heads} do not form a GQA group")
+        nq = heads * D * (2 if gated else 1)
+        if qkv.ndim != 2 or qkv.shape[1] != nq + 2 * kv_heads * D:
+            raise RuntimeError(f"qkv {tuple(qkv.shape)} is not (T, {nq + 2 * kv_heads * D})")
+        tokens = qkv.shape[0]
+        pages, size, groups, sp, st, sh = self._paged_kv(k, v, D)
+        if groups != kv_heads:
+            raise RuntimeError(f"the cache holds {groups} kv heads, not {kv_heads}")
+        self._check_table(table)
+        self._check_ints("pos", pos, tokens)
+        if rows is not None:
+            self._check_ints("rows", rows, tokens)
+        elif table.shape[0] < tokens:
+            raise RuntimeError("table needs a row per token where rows is not given")
+        if (q_norm is None) != (k_norm is None) or (cos is None) != (sin is None):
+            raise RuntimeError("q_norm and k_norm, and cos and sin, are given together")
+        if q_norm is not None:
+            self._check_f32_dev("q_norm", q_norm)
+            self._check_f32_dev("k_norm", k_norm)
+            if q_norm.numel() != D or k_norm.numel() != D:
+                raise ValueError("q_norm/k_norm must hold head_dim values")
+            q_norm, k_norm = q_norm.reshape(-1).contiguous(), k_norm.reshape(-1).contiguous()
+        cap = 1
+        if cos is not None:
+            rope_dim = operator.index(rope_dim)
+            if rope_dim < 2 or rope_dim % 2 or rope_dim > D:
+                raise ValueError(f"invalid rope_dim {rope_dim} for rows of {D}")
+            for n, t in (("cos", cos), ("sin", sin)):
+                self._check_f32_dev(n, t)
+                if t.ndim != 2 or t.shape[1] != rope_dim or not t.is_contiguous():
+                    raise RuntimeError(f"{n} must be a contiguous (cap, rope_dim) table")
+            if sin.shape != cos.shape or cos.shape[0] < 1:
+                raise RuntimeError("cos and sin tables differ in shape, or are empty")
+            cap = cos.shape[0]
+        self._on_device(qkv=qkv, pos=pos, rows=rows, k=k, v=v, table=table)
+        code, q_code = _dtype_code(qkv.dtype), _dtype_code(q_dtype)
+        if qkv.stride(1) != 1 or qkv.stride(0) < qkv.shape[1] or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+            qkv = qkv.contiguous()
+        q = torch.empty((tokens, heads, D), dtype=q_dtype, device=self._dev)
+        if tokens:
+            self._run("bt_attn_prep_paged", qkv.data_ptr(), code, qkv.stride(0), tokens, heads, kv_heads, D, int(gated),
+                      _ptr(q_norm), _ptr(k_norm), float(eps), _ptr(cos), _ptr(sin), rope_dim if cos is not None else 0,
+                      cap, int(interleaved), pos.data_ptr(), _ptr(rows), q.data_ptr(), q_code, k.data_ptr(),
+                      v.data_ptr(), sp, st, sh, pages, size, table.data_ptr(), table.shape[1], table.shape[0],
+                      table.shape[1])
+        return q, qkv[:, :nq].view(tokens, heads, 2 * D)[..., D:] if gated else None
+
+    def _page_args(self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor | None):
+        if pages.dtype is not torch.bfloat16 or pages.ndim != 4 or pages.shape[0] < 1 or pages.shape[1] < 1:
+            raise RuntimeError("pages must be a bf16 (planes, pages, page_size, Hkv * D) tensor")
+        planes, num, size, width = pages.shape
+        if size not in PAGE_SIZES:
+            raise RuntimeError(f"page size {size} is not served {PAGE_SIZES}")
+        if width < 8 or width % 8 or pages.stride(3) != 1 or pages.stride(2) != width:
+            raise RuntimeError("each page must be contiguous, Hkv * D a multiple of 8")
+        page_stride = pages.stride(1) if num > 1 else size * width
+        plane_stride = pages.stride(0) if planes > 1 else num * page_stride
+        self._check_table(table)
+        self._check_ints("lens", lens, table.shape[0])
+        if keep is not None:
+            self._check_ints("keep", keep, keep.numel())
+        self._on_device(pages=pages, table=table, lens=lens, keep=keep)
+        return pages.data_ptr(), plane_stride, page_stride, planes, num, size, width
+
+    def fork_pages(
+        self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent: torch.Tensor | None = None,
+        add: torch.Tensor | int = 0, keep: torch.Tensor | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Sequences that continue others, with room for their next tokens.
+
+        pages (planes, pages, page_size, Hkv * D) bf16 (``PagedKVCache.pages``); table
+        (R, P) and lens (R,) int32.  Row i of the result continues row parent[i]
+        (int32, any number of rows; default: itself; outside 0 .. R - 1: an empty row),
+        its pages shared, and has room for ``add`` more tokens ((rows,) int32 or one
+        number): free pages, lowest first, and a copy of the last page where that is
+        partly filled and held by another row or by ``keep`` (int32 page ids that must
+        stay).  A page no new row holds and ``keep`` does not name is free: sequences
+        end by having no child.  Returns (table, lens, status): new tensors, lens
+        without the added tokens, status (2,) int32 = pages left free and pages that
+        could not be given -- their entries are -1, and the old table still names
+        what the new rows would lose, so the step can be taken again."""
+        args = self._page_args(pages, table, lens, keep)
+        rows_in, per_seq = table.shape
+        rows = rows_in
+        if parent is not None:
+            rows = parent.numel()
+            self._check_ints("parent", parent, rows)
+        if not isinstance(add, torch.Tensor):
+            n = operator.index(add)
+            if not 0 <= n <= 0x7FFFFFFF:
+                raise ValueError(f"add must not be negative or over 2^31 - 1, got {n}")
+            add = torch.full((rows,), n, dtype=torch.int32, device=self._dev) if n else None
+        else:
+            self._check_ints("add", add, rows)
+        self._on_device(parent=parent, add=add)
+        new = torch.empty((rows, per_seq), dtype=torch.int32, device=self._dev)
+        new_lens = torch.empty(rows, dtype=torch.int32, device=self._dev)
+        status = torch.empty(2, dtype=torch.int32, device=self._dev)
+        nbytes = self._lib.bt_pages_workspace_bytes(args[4], max(rows, rows_in))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
+        self._run("bt_fork_pages", *args, table.data_ptr(), lens.data_ptr(), rows_in, per_seq, _ptr(parent), _ptr(add), rows,
+                  _ptr(keep), 0 if keep is None else keep.numel(), new.data_ptr(), new_lens.data_ptr(),
+                  status.data_ptr(), ws.data_ptr(), nbytes)
+        return new, new_lens, status
+
+    def compact_pages(
+        self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Live pages moved to the lowest places: those that the rows' tokens lie in or
+        ``keep`` names (arguments as ``fork_pages``).  Returns (table, where, live): the
+        new table, the new place of every page ((pages,) int32, -1: free; for other
+        tables and ``keep``), and the number of live pages ((1,) int32)."""
+        args = self._page_args(pages, table, lens, keep)
+        rows, per_seq = table.shape
+        new = torch.empty_like(table)
+        where = torch.empty(args[4], dtype=torch.int32, device=self._dev)
+        live = torch.empty(1, dtype=torch.int32, device=self._dev)
+        nbytes = self._lib.bt_pages_workspace_bytes(args[4], rows)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
+        self._run("bt_compact_pages", *args, table.data_ptr(), lens.data_ptr(), rows, per_seq, _ptr(keep),
+                  0 if keep is None else keep.numel(), new.data_ptr(), where.data_ptr(), live.data_ptr(), ws.data_ptr(),
+                  nbytes)
+        return new, where, live
+
+    def beam_select(
+        self, logits: torch.Tensor, scores: torch.Tensor, beams: int | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Beam search's selection: of scores[b, w] + log_softmax(logits[b, w])[v] the
+        best ``beams`` (default: as many as there are) of each b.
+
+        logits (B, W, V) f32 or bf16, scores (B, W) f32 -> (scores (B, beams) f32, best
+        first, parent (B, beams) int32, the row b * W + w each continues, token (B,
+        beams) int32).  Compared in 64 bits; ties go to the lower beam, then to the
+        lower token.  A barred token has the logit -inf (NaN counts as that); a beam
+        that has ended keeps its score with one logit of 0 and -inf elsewhere."""
+        if logits.ndim != 3 or scores.shape != logits.shape[:2]:
+            raise RuntimeError("beam_select expects logits (B, W, V) and scores (B, W)")
+        batch, width, vocab = logits.shape
+        beams = width if beams is None else operator.index(beams)
+        if vocab < 1 or width < 1 or not 1 <= beams <= width * vocab:
+            raise ValueError(f"{beams} beams cannot be taken from {width} x {vocab} candidates")
+        if width > MAX_BEAMS or beams > MAX_BEAMS:
+            raise RuntimeError(f"more than {MAX_BEAMS} beams are not served")
+        code = _dtype_code(logits.dtype)
+        self._check_f32_dev("scores", scores)
+        self._on_device(logits=logits)
+        if logits.stride(2) != 1:
+            logits = logits.contiguous()
+        scores = scores.contiguous()
+        best = torch.empty((batch, beams), dtype=torch.float32, device=self._dev)
+        parent = torch.empty((batch, beams), dtype=torch.int32, device=self._dev)
+        token = torch.empty((batch, beams), dtype=torch.int32, device=self._dev)
+        if batch == 0:
+            return best, parent, token
+        nbytes = self._lib.bt_beam_workspace_bytes(batch, width, vocab, beams)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
+        self._run("bt_beam_select", logits.data_ptr(), code, logits.stride(0), logits.stride(1), scores.data_ptr(), batch,
+                  width, vocab, beams, best.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), nbytes)
+        return best, parent, token
 
     def close(self) -> None:
         self._ws.clear()

@@ -390,4 +390,105 @@ hipError_t launch_attn_prep(const RowPrepParams& p, int head_dim, hipStream_t st
 hipError_t launch_gdn_decode(const GdnParams& p, int dim, hipStream_t stream);
 hipError_t launch_gemv(const GemvParams& p, const GemvShape& shape, hipStream_t stream);
 
+// ---------------------------------------------------------------- paged caches
+// A cache in pages: element (page, token, kv head, d) of k or v at page *
+// stride_page + token * stride_tok + head * stride_head + d; a sequence's token t
+// lies in page table[row * table_stride + t / page_size] at token t % page_size.
+struct PagedLayout {
+  int64_t stride_page, stride_tok, stride_head;
+  int32_t num_pages;
+  int32_t page_shift;       // log2(page_size)
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t pages_per_seq;
+};
+
+// Page sizes served: powers of two in this range.  16 is the decode tile, so a
+// tile never crosses a page.
+constexpr int kMinPageSize = 16, kMaxPageSize = 1024;
+inline bool page_size_served(int s) { return s >= kMinPageSize && s <= kMaxPageSize && (s & (s - 1)) == 0; }
+
+constexpr int kPagedMaxBatch = 4096;
+struct PagedDecodeParams {
+  const void* q;  // (batch, heads, D) f32 or bf16; head stride = D
+  int64_t q_stride_seq;
+  int q_bf16;
+  const uint16_t* k;
+  const uint16_t* v;
+  PagedLayout pg;
+  const int32_t* lens;  // (batch,) valid keys
+  int32_t batch, heads, kv_heads, group;
+  float scale_log2;
+  void* out;
+  int out_bf16;
+  int64_t out_stride_seq;
+};
+hipError_t launch_decode_paged(const PagedDecodeParams& p, int head_dim, hipStream_t stream);
+
+struct PagedPrepParams {
+  const void* x;  // (tokens, row): [heads x q (| gate) | kv_heads x k | kv_heads x v], f32 or bf16
+  int x_bf16;
+  int64_t x_stride;
+  int32_t tokens, heads, kv_heads, gated;
+  const float* wq;  // norm weights (D,), both or none
+  const float* wk;
+  float eps;
+  const float* cos;  // (rope_cap, rope_dim), both or none
+  const float* sin;
+  int32_t rope_dim, rope_cap, interleaved;
+  const int32_t* pos;   // (tokens,)
+  const int32_t* rows;  // (tokens,) table row, or null: token t writes row t
+  int32_t table_rows;
+  void* q_out;  // (tokens, heads, D)
+  int q_out_bf16;
+  uint16_t* k;
+  uint16_t* v;
+  PagedLayout pg;
+};
+hipError_t launch_paged_prep(const PagedPrepParams& p, int head_dim, hipStream_t stream);
+
+// Page operators: `pages` holds planes of num_pages pages of page_size tokens of
+// token_elems 16-bit values; a page is contiguous.
+struct PageOpParams {
+  uint16_t* pages;
+  int64_t plane_stride, page_stride;
+  int32_t planes, num_pages, page_size, token_elems;
+  const int32_t* table;  // (rows, pages_per_seq)
+  const int32_t* lens;   // (rows,)
+  int32_t rows, pages_per_seq;
+  const int32_t* parent;  // (rows_out,) or null: row i continues row i
+  const int32_t* add;     // (rows_out,) or null: none
+  int32_t rows_out;
+  const int32_t* keep;  // (num_keep,) pages held besides the rows'
+  int32_t num_keep;
+  int32_t* table_out;  // (rows_out, pages_per_seq)
+  int32_t* lens_out;   // fork: (rows_out,)
+  int32_t* status;     // fork: {pages left free, pages missing}; compact: {live pages}
+  int32_t* where;      // compact: (num_pages,) new place of each page, -1: free
+  int32_t* ws;         // page_ws_ints() values
+};
+// Workspace: a count per page, the free pages (compact: holes, then movers), and
+// the copies: their number, then {from, to, tokens} each.
+inline int64_t page_ws_ints(int64_t num_pages, int64_t rows_out) {
+  const int64_t copies = num_pages > rows_out ? num_pages : rows_out;
+  return 2 * num_pages + 4 + 4 * copies;
+}
+hipError_t launch_fork_pages(const PageOpParams& p, hipStream_t stream);
+hipError_t launch_compact_pages(const PageOpParams& p, hipStream_t stream);
+
+struct BeamParams {
+  const void* logits;  // (batch, width, vocab) f32 or bf16, unit vocab stride
+  int bf16;
+  int64_t stride_batch, stride_beam;
+  const float* scores;  // (batch, width)
+  int32_t batch, width, vocab, beams;
+  void* ws;  // beam_ws_bytes()
+  float* scores_out;   // (batch, beams)
+  int32_t* parent_out;  // (batch, beams): batch * width + beam
+  int32_t* token_out;
+};
+constexpr int kMaxBeams = 64, kMaxBeamWidth = 64;
+int64_t beam_ws_bytes(int batch, int width, int vocab, int beams);
+hipError_t launch_beam_select(const BeamParams& p, hipStream_t stream);
+
 }  // namespace bt

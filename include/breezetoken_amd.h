@@ -368,6 +368,115 @@ int bt_gemv_plan(const void* w, int64_t ldw, int32_t K, int32_t N, int32_t* plan
 int bt_gemv_bf16(const float* x, const void* w, int64_t ldw, int32_t K, int32_t N, float* y,
                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------ paged caches
+ *
+ * A cache in pages: num_pages pages of page_size tokens (a power of two, 16 to
+ * 1,024); element (page, token, kv_head, d) of the bf16 k or v at page *
+ * stride_page + token * stride_tok + kv_head * stride_head + d, strides
+ * positive multiples of 8 elements.  table (rows, pages_per_seq) int32, row
+ * stride table_stride, holds page ids: token t of a row lies in the page of
+ * entry t / page_size at token t % page_size.  Entries past a row's last token
+ * are not read; an entry outside [0, num_pages) holds no keys and takes no
+ * writes.  The reference has no counterpart (its cache is one contiguous array
+ * of one sequence, breezetoken/model/config.py:100-111). */
+
+/* Bytes of workspace bt_gqa_decode_paged needs on the current device for rows of
+ * up to max_tokens = pages_per_seq * page_size tokens (0: none). */
+int64_t bt_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                 int32_t max_tokens);
+
+/* Decode attention of one new token per sequence over a paged cache: sequence b
+ * attends the first lens[b] tokens of table row b (clamped to 0 ..
+ * pages_per_seq * page_size; none: zeros).  q (batch, heads, head_dim) f32 or
+ * bf16, out the same shape f32 or bf16.  head_dim in {64, 128, 256}, heads /
+ * kv_heads <= 8, batch <= 4,096.  A page may stand in several rows, or twice in
+ * one.  `workspace` is scratch for the duration of the call on `stream`: calls
+ * that may overlap need one each.  It generalises gqa_decode's split and combine
+ * (breezetoken/kernels/cuda/attention.py:54-205). */
+int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, const void* k, const void* v,
+                        int64_t stride_page, int64_t stride_tok, int64_t stride_head, int32_t num_pages,
+                        int32_t page_size, const int32_t* table, int64_t table_stride, int32_t pages_per_seq,
+                        const int32_t* lens, int32_t batch, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes, void* out,
+                        int32_t out_dtype, int64_t out_stride_seq, void* stream);
+
+/* Preparation of an attention layer over a paged cache, any number of tokens
+ * (those of a decode step or of whole prompts) in one launch: what bt_attn_prep
+ * does for one (breezetoken/model/layers.py:58-73, prefill.py:49-55).  qkv
+ * (tokens, row) f32 or bf16, row stride qkv_stride (a multiple of 8), holds
+ * [heads x q | kv_heads x k | kv_heads x v], with `gated` [heads x (q | gate) |
+ * ...].  q and k are normalised with q_norm / k_norm (head_dim,) f32 (both or
+ * neither), then their first rope_dim values rotated by row pos[t] of the cos /
+ * sin tables (rope_cap, rope_dim), clamped to the tables (both or neither):
+ * values i and i + rope_dim / 2 by column i, with `interleaved` values 2i and
+ * 2i + 1; columns past rope_dim / 2 are not read.  q goes to q_out (tokens,
+ * heads, head_dim) f32 or bf16, k and v to token pos[t] of table row rows[t]
+ * (rows NULL: row t), rounded to bf16; a row outside [0, table_rows), a
+ * position outside the row or an entry outside the cache writes neither.  Two
+ * tokens of one call must not name the same slot: which one it then holds is
+ * not defined.  head_dim in {64, 128, 256, 512}. */
+int bt_attn_prep_paged(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, int32_t tokens, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t gated, const float* q_norm,
+                       const float* k_norm, float eps, const float* cos, const float* sin, int32_t rope_dim,
+                       int32_t rope_cap, int32_t interleaved, const int32_t* pos, const int32_t* rows,
+                       void* q_out, int32_t q_dtype, void* k, void* v, int64_t stride_page,
+                       int64_t stride_tok, int64_t stride_head, int32_t num_pages, int32_t page_size,
+                       const int32_t* table, int64_t table_stride, int32_t table_rows, int32_t pages_per_seq,
+                       void* stream);
+
+/* Bytes of workspace bt_fork_pages and bt_compact_pages need, `rows` the larger of
+ * the rows they read and write. */
+int64_t bt_pages_workspace_bytes(int32_t num_pages, int32_t rows);
+
+/* Sequences that continue others in a paged cache, with room for their next
+ * tokens.  pages: planes (K and V of every layer) of num_pages contiguous pages
+ * of page_size * token_elems bf16 values, plane and page strides in elements.
+ * table (rows, pages_per_seq) and lens (rows,) are the cache before; row i of
+ * table_out (rows_out, pages_per_seq) and lens_out (rows_out,) continues row
+ * parent[i] with its length, or is empty where that is outside [0, rows)
+ * (parent NULL: row i, rows_out = rows or 0).  Its entries up to add[i] more tokens
+ * (add NULL: none) hold pages, the further ones -1: pages no new row holds, nor
+ * `keep` (num_keep ids), lowest first, in row order.  Where add[i] > 0 and the
+ * last page is partly filled and held more than once, its tokens are copied to a
+ * fresh page in every plane.  table and lens stay as they are and must not
+ * overlap the outputs.  status (2,): pages left free, and pages that could not be
+ * given (too few pages or entries): those entries are -1, the row's tokens in
+ * them lost to the new row, but not to the old one.  No reference counterpart. */
+int bt_fork_pages(void* pages, int64_t plane_stride, int64_t page_stride, int32_t planes, int32_t num_pages,
+                  int32_t page_size, int32_t token_elems, const int32_t* table, const int32_t* lens,
+                  int32_t rows, int32_t pages_per_seq, const int32_t* parent, const int32_t* add,
+                  int32_t rows_out, const int32_t* keep, int32_t num_keep, int32_t* table_out,
+                  int32_t* lens_out, int32_t* status, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Live pages moved to the lowest places: the n pages that rows or `keep` hold
+ * become pages 0 .. n - 1, those already there stay, the others fill the free
+ * places in order.  table_out (rows, pages_per_seq) names the new places (-1 past
+ * a row's last page), where (num_pages,) the new place of every page (-1: free),
+ * live (1,) their number.  No reference counterpart. */
+int bt_compact_pages(void* pages, int64_t plane_stride, int64_t page_stride, int32_t planes,
+                     int32_t num_pages, int32_t page_size, int32_t token_elems, const int32_t* table,
+                     const int32_t* lens, int32_t rows, int32_t pages_per_seq, const int32_t* keep,
+                     int32_t num_keep, int32_t* table_out, int32_t* where, int32_t* live, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace bt_beam_select needs. */
+int64_t bt_beam_workspace_bytes(int32_t batch, int32_t width, int32_t vocab, int32_t beams);
+
+/* Beam search's selection: the best `beams` of each batch item's width * vocab
+ * continuations scores[b, w] + logits[b, w, v] - log(sum_u exp(logits[b, w, u])).
+ * logits (batch, width, vocab) f32 or bf16, unit vocab stride; scores (batch,
+ * width) f32.  scores_out (batch, beams) f32, best first; parent_out the row b *
+ * width + w that each continues (bt_fork_pages' parent), token_out its token.
+ * Sums and comparisons are in 64 bits: a beam's candidates go by their logits,
+ * equal ones by token, those of two beams by value, equal ones by beam.  A NaN
+ * logit counts as -inf; candidates of -inf are chosen only when no others are
+ * left.  width and beams <= 64, beams <= width * vocab.  The reference decodes
+ * greedily (breezetoken/model/graph.py:87-91). */
+int bt_beam_select(const void* logits, int32_t dtype, int64_t stride_batch, int64_t stride_beam,
+                   const float* scores, int32_t batch, int32_t width, int32_t vocab, int32_t beams,
+                   float* scores_out, int32_t* parent_out, int32_t* token_out, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
