@@ -56,6 +56,7 @@ struct CombineParams {
   int32_t total_splits;
   const int32_t* split_base;    // (batch,) first split of each sequence, or null
   const int32_t* split_count;   // (batch,) splits of each sequence, or null
+  int32_t skip_single;          // 1: a sequence of one split has its result already
   void* out;                    // (batch, heads, D)
   int out_bf16;
   int64_t out_stride_seq;
@@ -419,10 +420,20 @@ struct PagedDecodeParams {
   const int32_t* lens;  // (batch,) valid keys
   int32_t batch, heads, kv_heads, group;
   float scale_log2;
+  int32_t runs;  // work-groups per kv head, paged_runs()
+  // Parts of sequences that lie in several runs (runs > 1): rows of runs + batch
+  // slots per head, and each sequence's first slot and their number.
+  float* lse;
+  float* part;
+  int32_t* part_base;
+  int32_t* part_count;
   void* out;
   int out_bf16;
   int64_t out_stride_seq;
 };
+// Fewest tiles a work-group takes: short contexts run on fewer work-groups.
+constexpr int kPagedTilesPerRun = 2;
+int paged_runs(int batch, int kv_heads, int head_dim, int64_t max_tokens, int num_cus);
 hipError_t launch_decode_paged(const PagedDecodeParams& p, int head_dim, hipStream_t stream);
 
 struct PagedPrepParams {

@@ -4,6 +4,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/breezetoken_amd.h"
 #include "bt_kernels.h"
 
@@ -14,6 +16,7 @@ constexpr double kLog2e = 1.4426950408889634;
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline bool dtype_known(int32_t t) { return t == BT_DTYPE_F32 || t == BT_DTYPE_BF16; }
+inline int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
 inline int hip_rc(hipError_t e) { return e == hipSuccess ? BT_OK : (int)e; }
 inline int log2_of(int32_t x) {
   int n = 0;
@@ -23,10 +26,11 @@ inline int log2_of(int32_t x) {
 
 // Pages and table of a cache.
 int check_paged(const void* k, const void* v, int64_t stride_page, int64_t stride_tok, int64_t stride_head,
-                int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_stride, int32_t pages_per_seq) {
+                int32_t num_pages, int32_t page_size, int32_t head_dim, const int32_t* table, int64_t table_stride,
+                int32_t pages_per_seq) {
   if (!k || !v || !table || !aligned16(k) || !aligned16(v) || !aligned4(table)) return BT_EINVAL;
   if (num_pages < 1 || pages_per_seq < 1 || table_stride < pages_per_seq) return BT_EINVAL;
-  if (stride_page < 8 || stride_tok < 8 || stride_head < 8 || stride_page % 8 || stride_tok % 8 || stride_head % 8)
+  if (stride_page < head_dim || stride_tok < head_dim || stride_head < head_dim || stride_page % 8 || stride_tok % 8 || stride_head % 8)
     return BT_EINVAL;
   if (!bt::page_size_served(page_size)) return BT_ENOTSUP;
   if ((int64_t)pages_per_seq * page_size > INT32_MAX - bt::kMaxPageSize) return BT_ENOTSUP;
@@ -48,13 +52,42 @@ bt::PagedLayout paged_layout(int64_t stride_page, int64_t stride_tok, int64_t st
   return l;
 }
 
+// Compute units of the current device.
+int device_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  static std::atomic<int> cache[64];
+  if (dev >= 0 && dev < 64 && (n = cache[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+  if (dev >= 0 && dev < 64) cache[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Decode workspace, each part 256-byte aligned: the parts' LSEs, the parts, and
+// each sequence's first slot and count.
+struct PagedWorkspace {
+  int32_t runs;
+  int64_t part, base, count, bytes;
+};
+PagedWorkspace paged_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens) {
+  PagedWorkspace w{};
+  w.runs = bt::paged_runs(batch, kv_heads, head_dim, max_tokens, device_cus());
+  if (w.runs == 1) return w;
+  const int64_t slots = (int64_t)heads * (w.runs + batch);
+  w.part = align256(slots * 4);
+  w.base = w.part + align256(slots * head_dim * 4);
+  w.count = w.base + align256((int64_t)batch * 4);
+  w.bytes = w.count + align256((int64_t)batch * 4);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t bt_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_tokens) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_tokens < 1) return 0;
-  return 0;
+  return paged_workspace(batch, heads, kv_heads, head_dim, max_tokens).bytes;
 }
 
 int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, const void* k, const void* v,
@@ -68,13 +101,16 @@ int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, co
   if (!dtype_known(q_dtype) || !dtype_known(out_dtype)) return BT_EINVAL;
   if (q_stride_seq < (int64_t)heads * head_dim || q_stride_seq % 8) return BT_EINVAL;
   if (out_stride_seq < (int64_t)heads * head_dim || out_stride_seq % 8) return BT_EINVAL;
-  int rc = check_paged(k, v, stride_page, stride_tok, stride_head, num_pages, page_size, table, table_stride, pages_per_seq);
+  int rc = check_paged(k, v, stride_page, stride_tok, stride_head, num_pages, page_size, head_dim, table, table_stride,
+                       pages_per_seq);
   if (rc) return rc;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return BT_ENOTSUP;
   if (heads / kv_heads > 8 || batch > bt::kPagedMaxBatch || kv_heads > 65535) return BT_ENOTSUP;
   if ((int64_t)batch * heads > INT32_MAX / 2) return BT_ENOTSUP;
-  const int64_t need = bt_paged_workspace_bytes(batch, heads, kv_heads, head_dim, pages_per_seq * page_size);
-  if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return BT_ENOSPC;
+  const int64_t max_tokens = (int64_t)pages_per_seq * page_size;
+  if (batch * (max_tokens / 16) > INT32_MAX / 2) return BT_ENOTSUP;  // tiles are numbered through the batch
+  const PagedWorkspace ws = paged_workspace(batch, heads, kv_heads, head_dim, max_tokens);
+  if (ws.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < ws.bytes)) return BT_ENOSPC;
   bt::PagedDecodeParams p{};
   p.q = q;
   p.q_stride_seq = q_stride_seq;
@@ -88,6 +124,14 @@ int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, co
   p.kv_heads = kv_heads;
   p.group = heads / kv_heads;
   p.scale_log2 = (float)((double)scale * kLog2e);
+  p.runs = ws.runs;
+  if (ws.bytes) {
+    char* at = static_cast<char*>(workspace);
+    p.lse = reinterpret_cast<float*>(at);
+    p.part = reinterpret_cast<float*>(at + ws.part);
+    p.part_base = reinterpret_cast<int32_t*>(at + ws.base);
+    p.part_count = reinterpret_cast<int32_t*>(at + ws.count);
+  }
   p.out = out;
   p.out_bf16 = out_dtype == BT_DTYPE_BF16;
   p.out_stride_seq = out_stride_seq;
@@ -110,7 +154,8 @@ int bt_attn_prep_paged(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, i
   if (q_norm && (!aligned16(q_norm) || !aligned16(k_norm))) return BT_EINVAL;
   if (cos && (rope_dim < 2 || rope_dim % 2 || rope_dim > head_dim || rope_cap < 1)) return BT_EINVAL;
   if (!(eps >= 0.f)) return BT_EINVAL;
-  int rc = check_paged(k, v, stride_page, stride_tok, stride_head, num_pages, page_size, table, table_stride, pages_per_seq);
+  int rc = check_paged(k, v, stride_page, stride_tok, stride_head, num_pages, page_size, head_dim, table, table_stride,
+                       pages_per_seq);
   if (rc) return rc;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) return BT_ENOTSUP;
   if ((int64_t)tokens * (heads + 2 * (int64_t)kv_heads) > INT32_MAX / 64) return BT_ENOTSUP;

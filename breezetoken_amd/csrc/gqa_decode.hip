@@ -37,51 +37,14 @@
 //    device length table, so the launch shape never depends on host data and the
 //    whole call can be captured in a hipGraph.
 #include "bt_common.h"
+#include "bt_decode.h"
 #include "bt_kernels.h"
 
 namespace bt {
 
 namespace {
 
-__device__ __forceinline__ int swz(int row, int slots) { return ((row & 7) * 2) & (slots - 1); }
-
-template <int V>
-struct IntConst {
-  static constexpr int value = V;
-};
-
-// Raw buffer resource over [base, base + bytes): loads past the end return 0,
-// so tokens past the valid length need no clamping.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
-}
 constexpr float kDecodeLazy = 8.0f;  // log2-domain slack before the reference max moves
-
-// K/V are streamed once per call: the non-temporal policy (nt) keeps them from
-// displacing reusable lines and measurably raises the stream rate on gfx950.
-constexpr int kPolicyStream = 2;  // gfx940+ cache-policy bits: nt
-__device__ __forceinline__ u32x4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
-  return __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, kPolicyStream);
-}
-
-typedef short short4_t __attribute__((ext_vector_type(4)));
-
-// Scalar (constant-cache) read of a wave-uniform value written by an earlier
-// kernel: issued as s_load, so its wait lands at the first use instead of
-// forcing a vector load + readfirstlane right away.
-template <typename T>
-__device__ __forceinline__ T uniform_load(const T* p, int i) {
-  return ((const __attribute__((address_space(4))) T*)(p))[i];
-}
-
-__device__ __forceinline__ floatx4 mfma16k16(const u32x2& a, const u32x2& b, const floatx4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a),
-                                                  __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
-}
-
-__device__ __forceinline__ u32x2 lds_read_tr4(const BT_LDS uint16_t* p) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((BT_LDS bf16x4*)p));
-}
 
 template <int GMAX>
 __device__ __forceinline__ float mirror(float v) {
@@ -590,7 +553,8 @@ __global__ __launch_bounds__(W * 64, 1) void gqa_decode_split_kernel(DecodeSplit
 // with it, against 17.17 us with 16 groups x 4 columns, 17.18 us with 64
 // groups x 1 column, and 17.68 us for a 256-thread work-group per 64-column
 // chunk with LDS reductions.
-template <int D, bool RAGGED, int GROUPS>
+// SKIP: a sequence of one split has its result already (the paged decode).
+template <int D, bool RAGGED, int GROUPS, bool SKIP = false>
 __global__ __launch_bounds__(64) void gqa_decode_combine_kernel(CombineParams p) {
   static_assert(GROUPS >= 1 && GROUPS <= 64 && (GROUPS & (GROUPS - 1)) == 0,
                 "split groups are a power of two that divides the 64 lanes");
@@ -604,6 +568,7 @@ __global__ __launch_bounds__(64) void gqa_decode_combine_kernel(CombineParams p)
   if constexpr (RAGGED) {
     base = p.split_base[b];
     ns = p.split_count[b];
+    if (SKIP && ns == 1) return;
   } else {
     base = b * p.num_split;
     ns = p.num_split;
@@ -771,7 +736,8 @@ template <int D>
 static void launch_combine_t(const CombineParams& p, int heads, int batch, hipStream_t stream) {
   if (p.split_base != nullptr) {
     const dim3 grid(heads, batch, D / (4 * (64 / kCombineRaggedGroups)));
-    hipLaunchKernelGGL((gqa_decode_combine_kernel<D, true, kCombineRaggedGroups>), grid, dim3(64), 0, stream, p);
+    if (p.skip_single) hipLaunchKernelGGL((gqa_decode_combine_kernel<D, true, kCombineRaggedGroups, true>), grid, dim3(64), 0, stream, p);
+    else hipLaunchKernelGGL((gqa_decode_combine_kernel<D, true, kCombineRaggedGroups>), grid, dim3(64), 0, stream, p);
   } else {
     const dim3 grid(heads, batch, D / (4 * (64 / kCombineGroups)));
     hipLaunchKernelGGL((gqa_decode_combine_kernel<D, false, kCombineGroups>), grid, dim3(64), 0, stream, p);

@@ -5,87 +5,517 @@
 //   out = sum_j exp2(x_j - m) v_j / l,  zeros for a sequence without keys
 //
 // A table entry outside [0, num_pages) holds no keys.
+//
+// Bound by the stream of K and V.  The batch's tiles (16 tokens each, never
+// across a page) are numbered through, sequence after sequence, and every
+// work-group of a kv head takes an equal run of them, whatever sequences it
+// falls into: all CUs stream the same number of bytes for any mix of lengths,
+// with no plan, no host lengths and no rounds of work-groups.  A run that covers
+// a sequence writes its result; the parts of a sequence cut by a run's end go to
+// the workspace as (lse, normalised partial) and the combine joins them.  The
+// part of work-group w in sequence b has slot w + b: runs and sequences both
+// advance in order, so slots are unique and a sequence's are consecutive.
+//
+// Within a work-group the waves take a run's tiles in turn, each with an online
+// softmax of its own, merged through LDS where a sequence ends.  A wave's next
+// tile -- K, V, and the page id of the one after -- is on its way while it works
+// on the current one, also across the end of a sequence, so the merge and the
+// next sequence's queries hide behind the stream.
+//
+// The MFMA takes K as it is and the query heads of the group as columns.  f32
+// queries and probabilities enter as sums of bf16 terms in further columns (and,
+// for 5 to 8 heads, a second MFMA): three terms hold all 24 bits where the output
+// is f32, two leave 2^-16 where it is rounded to bf16 (2^-8).
 #include "bt_common.h"
+#include "bt_decode.h"
 #include "bt_kernels.h"
 
 namespace bt {
 
 namespace {
 
-// One work-group of four waves per (sequence, query head); wave w takes the
-// tokens w, w + 4, ...; lane l holds the dims l, l + 64, ...
-template <int D, bool QBF16>
-__global__ __launch_bounds__(256) void gqa_paged_kernel(PagedDecodeParams p) {
-  constexpr int E = D / 64;
-  const int h = (int)blockIdx.x % p.heads, b = (int)blockIdx.x / p.heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int kvh = h / p.group;
-  const int64_t cap = (int64_t)p.pg.pages_per_seq << p.pg.page_shift;
-  int64_t valid = p.lens[b];
-  if (valid > cap) valid = cap;
-  float q[E], o[E];
+constexpr int kWaves = 8;
+constexpr float kLazy = 8.0f;  // log2-domain slack before the reference max moves: probabilities stay below 2^8
+
+// Sum over the column groups of 16 / GMAX that hold the terms of one head: every
+// column gets its head's sum.
+template <int GMAX>
+__device__ __forceinline__ float term_sum(float v) {
+  v += dpp_f32<0x128>(v);  // row_ror:8
+  if constexpr (GMAX == 4) v += dpp_f32<0x124>(v);  // row_ror:4
+  return v;
+}
+
+// The 16-byte slot of a tile's row that holds chunk c is c ^ slot_of(row): linear in
+// the row's bits, and such that the operand reads of K (16 rows, one chunk) and the
+// transposed reads of V (8 rows, a pair of chunks) fall on distinct banks.
+template <int D>
+__device__ __forceinline__ constexpr int slot_of(int r) {
+  return D == 64 ? (r >> 1 & 3) << 1 | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
+}
+
+__device__ __forceinline__ int bcast(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// 64 sequences' lengths and the batch-wide number of their last tile + 1.
+struct Window {
+  int first;  // sequence of lane 0
+  int start;  // tiles before it
+  int len, ends;
+  __device__ __forceinline__ void load(const PagedDecodeParams& p, int f, int s, int cap) {
+    first = f;
+    start = s;
+    const int b = f + (int)(threadIdx.x & 63);
+    len = b < p.batch ? p.lens[b] : 0;
+    len = len < 0 ? 0 : (len > cap ? cap : len);
+    int x = (len + 15) >> 4;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int64_t at = (int64_t)b * p.q_stride_seq + (int64_t)h * D + e * 64 + lane;
-    q[e] = QBF16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.q)[at]) : reinterpret_cast<const float*>(p.q)[at];
-    q[e] *= p.scale_log2;
-    o[e] = 0.f;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o);
+      if ((int)(threadIdx.x & 63) >= o) x += y;
+    }
+    ends = s + x;
   }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = wave; j < valid; j += 4) {
-    const int page = p.pg.table[(int64_t)b * p.pg.table_stride + (j >> p.pg.page_shift)];
-    if (page < 0 || page >= p.pg.num_pages) continue;
-    const int64_t row = (int64_t)page * p.pg.stride_page + (j & ((1 << p.pg.page_shift) - 1)) * p.pg.stride_tok +
-                        (int64_t)kvh * p.pg.stride_head;
-    float x = 0.f;
+  // The lane whose sequence holds tile t (64: a later window).
+  __device__ __forceinline__ int find(int t) const { return __popcll(__builtin_amdgcn_ballot_w64(ends <= t)); }
+  __device__ __forceinline__ int begin(int lane) const { return lane ? bcast(ends, lane - 1) : start; }
+};
+
+template <int GMAX, int D, bool QBF16, bool F32OUT>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kernel(PagedDecodeParams p) {
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kSteps = D / 32;
+  constexpr int kDTiles = D / 16;
+  constexpr int kSlots = D / 8;
+  constexpr int kRowBytes = D * 2;
+  constexpr int kTileBytes = 16 * kRowBytes;
+  constexpr int kLoads = kTileBytes / 1024;  // 1 KiB wave loads per K or V tile
+  constexpr int kRowsPerLoad = 1024 / kRowBytes;
+  constexpr int kGroups = 16 / GMAX;                  // column groups
+  constexpr int kTerms = F32OUT ? 3 : 2;
+  constexpr bool kSecond = kTerms > kGroups;          // the third term in an MFMA of its own
+  constexpr int kMoStride = D + 4;
+  static_assert(kSteps == kLoads && kSteps <= kWaves, "one wave per d-step builds Q^T");
+
+  __shared__ __attribute__((aligned(1024))) unsigned char tiles_lds[kWaves * kTileBytes];
+  __shared__ __attribute__((aligned(16))) float mlds[kWaves * GMAX * kMoStride];
+  __shared__ __attribute__((aligned(16))) u32x4 qlds[(kSecond ? 2 : 1) * kSteps * 64];
+  __shared__ float mstat[2 * kWaves * GMAX];
+  __shared__ int wsum[64];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = (int)blockIdx.x % p.kv_heads, w = (int)blockIdx.x / p.kv_heads;
+  const int G = p.group, head0 = kvh * G;
+  const int cap = p.pg.pages_per_seq << p.pg.page_shift;
+
+  // ---- the batch's tiles and this work-group's run ---------------------------
+  const int windows = (p.batch + 63) >> 6;  // at most 64
+  Window win;  // of the tile looked at last
+  int wends = 0, total;
+  if (windows == 1) {
+    win.load(p, 0, 0, cap);
+    total = bcast(win.ends, 63);
+  } else {
+    for (int i = wave; i < windows; i += kWaves) {
+      win.load(p, 64 * i, 0, cap);
+      if (lane == 63) wsum[i] = win.ends;
+    }
+    __syncthreads();
+    wends = lane < windows ? wsum[lane] : 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x = fmaf(q[e], bf16_bits_to_f32(p.k[row + e * 64 + lane]), x);
-    x = wave_sum(x);
-    const float mn = fmax_nc(m, x);  // a NaN score makes the row NaN
-    const float a = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(x - mn);
-    m = mn;
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(w, bf16_bits_to_f32(p.v[row + e * 64 + lane]), o[e] * a);
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(wends, o);
+      if (lane >= o) wends += y;
+    }
+    total = bcast(wends, 63);
+    win.first = -1;
   }
-  __shared__ float ms[4], ls[4], os[4][D];
-  if (lane == 0) {
-    ms[wave] = m;
-    ls[wave] = l;
+  // To the window that holds tile t < total.
+  auto seek = [&](int t) {
+    if (windows == 1) return;
+    const int i = __popcll(__builtin_amdgcn_ballot_w64(wends <= t));
+    if (win.first != 64 * i) win.load(p, 64 * i, i ? bcast(wends, i - 1) : 0, cap);
+  };
+  int runs = (total + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
+  runs = runs < 1 ? 1 : (runs < p.runs ? runs : p.runs);
+  const int share = total ? (total + runs - 1) / runs : 1;
+  const int t0 = w * share < total ? w * share : total;
+  const int t1 = t0 + share < total ? t0 + share : total;
+
+  // The last work-group of the first head, often an idle one, says where each
+  // sequence's parts are: their number (1: the result is written) and first slot.
+  if (w == p.runs - 1 && kvh == 0 && p.runs > 1) {
+    for (int i = wave; i < windows; i += kWaves) {
+      if (windows > 1) win.load(p, 64 * i, i ? bcast(wends, i - 1) : 0, cap);
+      const int b = 64 * i + lane, n = (win.len + 15) >> 4;
+      if (b < p.batch) {
+        const int w0 = (win.ends - n) / share;
+        p.part_base[b] = w0 + b;
+        p.part_count[b] = n ? (win.ends - 1) / share - w0 + 1 : 0;
+      }
+    }
   }
+
+  const int64_t head_off = (int64_t)kvh * p.pg.stride_head;
+  auto store_out = [&](int b, int h, int d, const float4& a) {
+    const int64_t row = (int64_t)b * p.out_stride_seq + (int64_t)(head0 + h) * D + d;
+    if (p.out_bf16) {
+      const u32x2 pk = {f32x2_to_bf16x2_bits(a.x, a.y), f32x2_to_bf16x2_bits(a.z, a.w)};
+      *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + row) = pk;
+    } else {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row) = a;
+    }
+  };
+  if (p.runs == 1) {  // no combine follows: sequences without keys are zeroed here
+    for (int i = 0; i < p.batch * G * (D / 4); i += kThreads) {
+      const int item = i + threadIdx.x, b = item / (G * (D / 4)), r = item % (G * (D / 4));
+      if (b < p.batch && p.lens[b] <= 0) store_out(b, r / (D / 4), r % (D / 4) * 4, float4{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+  if (t0 >= t1) return;
+
+  // ---- columns: head col % GMAX, term col / GMAX -------------------------------
+  const int col = lane & 15, kg = lane >> 4;
+  const int col_head = col & (GMAX - 1), term = col / GMAX;
+  // A value's terms as packed bf16: this lane's, and (second) the third one for the first columns.
+  const uint32_t keep0 = term == 0 && col_head < G ? 0xffffffffu : 0u;
+  const uint32_t keep1 = term == 1 && col_head < G ? 0xffffffffu : 0u;
+  const uint32_t keep2 = !kSecond && kTerms == 3 && term == 2 && col_head < G ? 0xffffffffu : 0u;
+  auto terms2 = [&](float a, float b, uint32_t& second) -> uint32_t {
+    const uint32_t h = f32x2_to_bf16x2_bits(a, b);
+    a -= __uint_as_float(h << 16);
+    b -= __uint_as_float(h & 0xffff0000u);
+    const uint32_t m = f32x2_to_bf16x2_bits(a, b);
+    uint32_t r = (h & keep0) | (m & keep1);
+    if constexpr (kTerms == 3) {
+      const uint32_t l = f32x2_to_bf16x2_bits(a - __uint_as_float(m << 16), b - __uint_as_float(m & 0xffff0000u));
+      if constexpr (kSecond) second = l & keep0;
+      else r |= l & keep2;
+    }
+    return r;
+  };
+
+  // ---- K/V tiles --------------------------------------------------------------
+  const uint32_t row_bytes = (uint32_t)(p.pg.stride_tok * 2);
+  unsigned char* tile_lds = tiles_lds + wave * kTileBytes;
+  // Load j of a tile fetches whole rows j * kRowsPerLoad + lane / kSlots; chunk c of row
+  // r goes to slot c ^ slot_of(r).  The part of the slot that depends on j is a constant,
+  // so an offset is one exclusive-or with it and one addition.
+  constexpr int kHiRows = kRowsPerLoad;  // rows of one load: a power of two
+  const uint32_t lane_slot = (uint32_t)((lane % kSlots) ^ slot_of<D>(lane / kSlots)) * 16;
+  const uint32_t lane_row = (uint32_t)(lane / kSlots) * row_bytes;
+  uint32_t load_base = lane_slot;
+  auto offset = [&](int j) -> uint32_t { return (load_base ^ (uint32_t)(slot_of<D>(j * kHiRows) * 16)) + lane_row; };
+  u32x4 kr[kSteps], vr[kLoads];
+  __amdgpu_buffer_rsrc_t krs, vrs;
+  auto issue_k = [&]() {
+    asm volatile("" : "+v"(load_base));  // offsets are made where they are used: sixteen fewer registers through the loop
 #pragma unroll
-  for (int e = 0; e < E; ++e) os[wave][e * 64 + lane] = o[e];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < 4; ++w) top = fmax_nc(top, ms[w]);
-  for (int w = 0; w < 4; ++w) sum += ms[w] == -INFINITY ? 0.f : ls[w] * exp2f(ms[w] - top);
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float y = 0.f;
-    for (int w = 0; w < 4; ++w) y += ms[w] == -INFINITY ? 0.f : os[w][d] * exp2f(ms[w] - top);
-    y = sum == 0.f ? 0.f : y / sum;
-    const int64_t at = (int64_t)b * p.out_stride_seq + (int64_t)h * D + d;
-    if (p.out_bf16) reinterpret_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16_bits(y);
-    else reinterpret_cast<float*>(p.out)[at] = y;
+    for (int j = 0; j < kLoads; ++j) kr[j] = buf_load16(krs, offset(j), (uint32_t)(j * kRowsPerLoad) * row_bytes);
+  };
+  auto issue_v = [&]() {
+    asm volatile("" : "+v"(load_base));
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) vr[j] = buf_load16(vrs, offset(j), (uint32_t)(j * kRowsPerLoad) * row_bytes);
+  };
+  // A tile to come: its page id (on its way), rows with keys, and first token in the page.
+  struct Tile {
+    int id, rows, token;
+  };
+  auto look_up = [&](int t) -> Tile {
+    Tile x{-1, 0, 0};
+    if (t < t1) {
+      seek(t);
+      const int i = win.find(t);
+      const int at = (t - win.begin(i)) * 16, b = win.first + i;
+      const int left = bcast(win.len, i) - at;
+      x.rows = left < 16 ? left : 16;
+      x.token = at & ((1 << p.pg.page_shift) - 1);
+      x.id = p.pg.table[(int64_t)b * p.pg.table_stride + (at >> p.pg.page_shift)];
+    }
+    return x;
+  };
+  // Points the tile's buffers at its page; returns the rows with keys.
+  auto open = [&](const Tile& x) -> int {
+    const int id = __builtin_amdgcn_readfirstlane(x.id);
+    const bool ok = id >= 0 && id < p.pg.num_pages;
+    const int rows = ok ? x.rows : 0;
+    const int64_t off = ok ? (int64_t)id * p.pg.stride_page + (int64_t)x.token * p.pg.stride_tok + head_off : 0;
+    krs = make_rsrc(p.k + off, (uint32_t)rows * row_bytes);
+    vrs = make_rsrc(p.v + off, (uint32_t)rows * row_bytes);
+    return rows;
+  };
+
+  // ---- queries of a sequence: raw values, then the Q^T operand ------------------
+  u32x4 qraw[2];
+  auto load_q = [&](int b) {
+    if (wave < kSteps) {
+      const int64_t row = (int64_t)b * p.q_stride_seq + (int64_t)(head0 + (col_head < G ? col_head : 0)) * D + (wave * 4 + kg) * 8;
+      if constexpr (QBF16) {
+        qraw[0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + row);
+      } else {
+        qraw[0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.q) + row);
+        qraw[1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.q) + row + 4);
+      }
+    }
+  };
+  auto build_q = [&]() {
+    if (wave < kSteps) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (QBF16) {
+          v[2 * i] = bf16_bits_to_f32(qraw[0][i] & 0xffffu);
+          v[2 * i + 1] = bf16_bits_to_f32(qraw[0][i] >> 16);
+        } else {
+          v[i] = __uint_as_float(qraw[0][i]);
+          v[4 + i] = __uint_as_float(qraw[1][i]);
+        }
+      }
+      u32x4 a, b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t second = 0;
+        a[i] = terms2(v[2 * i] * p.scale_log2, v[2 * i + 1] * p.scale_log2, second);
+        b[i] = second;
+      }
+      qlds[wave * 64 + lane] = a;
+      if constexpr (kSecond) qlds[(kSteps + wave) * 64 + lane] = b;
+    }
+  };
+
+  // ---- first tile of this wave, and the id of its second -------------------------
+  int t = t0 + wave;
+  seek(t0);
+  load_q(win.first + win.find(t0));
+  Tile cur = look_up(t), next = look_up(t + kWaves);
+  int rows = 0;
+  if (t < t1) {
+    rows = open(cur);
+    issue_k();
+    issue_v();
+  }
+
+  const int i16 = lane & 15;
+  const int row1 = 4 * kg + (i16 >> 2);  // V^T read: token row of this lane
+  // LDS addresses of the operand reads of step / d-tile 0; those of the others differ in
+  // bits of their own (rows are powers of two, slots are exclusive-ors), so they are made
+  // by an exclusive-or where they are used and take no registers through the loop.
+  const uint32_t tile_at = (uint32_t)(uintptr_t)(BT_LDS unsigned char*)tile_lds;
+  uint32_t k_at = tile_at + col * kRowBytes + ((kg ^ slot_of<D>(col)) * 16);
+  uint32_t v_at = tile_at + row1 * kRowBytes + ((((i16 & 3) >> 1) ^ slot_of<D>(row1)) * 16) + (i16 & 1) * 8;
+  for (int s0 = t0; s0 < t1;) {
+    // ---- one sequence's part: tiles [s0, s1) -------------------------------------
+    seek(s0);
+    const int lane_b = win.find(s0), b = win.first + lane_b;
+    const int seq_begin = win.begin(lane_b), seq_end = bcast(win.ends, lane_b);
+    const int s1 = seq_end < t1 ? seq_end : t1;
+    build_q();
+    // Also: every thread is done with the merge of the part before.
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    floatx4 oacc[kDTiles];
+#pragma unroll
+    for (int i = 0; i < kDTiles; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+    for (; t < s1; t += kWaves) {
+      const bool more = t + kWaves < t1;
+      // S^T = K . Q^T, K through the wave's tile into the operand layout.
+      floatx4 sacc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+        *reinterpret_cast<BT_LDS u32x4*>((BT_LDS unsigned char*)tile_lds + j * 1024 + lane * 16) = kr[j];
+      int next_rows = 0;
+      if (more) {
+        next_rows = open(next);
+        issue_k();
+      }
+      u32x4 kop[kSteps];
+      asm volatile("" : "+v"(k_at), "+v"(v_at));
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) kop[st] = *reinterpret_cast<const BT_LDS u32x4*>(k_at ^ (uint32_t)(st * 64));
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const u32x4 q = qlds[st * 64 + lane];
+        sacc = mfma16(as_bf16x8(kop[st]), as_bf16x8(q), sacc);
+        if constexpr (kSecond) sacc = mfma16(as_bf16x8(kop[st]), as_bf16x8(qlds[(kSteps + st) * 64 + lane]), sacc);
+      }
+      // V into the wave's tile behind K's reads (one wave's LDS operations stay in order).
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        *reinterpret_cast<BT_LDS u32x4*>((BT_LDS unsigned char*)tile_lds + j * 1024 + lane * 16) = vr[j];
+      if (more) {
+        issue_v();
+        next = look_up(t + 2 * kWaves);
+      }
+      // Terms summed, rows without a key masked, online softmax.
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = term_sum<GMAX>(sacc[j]);
+        x[j] = kg * 4 + j < rows ? v : -INFINITY;
+      }
+      float tmax = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      tmax = rows16_fmaxf(tmax);
+      tmax = halves_fmaxf(tmax);
+      // The reference max moves only when a score exceeds it by 2^8, so O and l are
+      // rescaled almost never; lse = log2(l) + m is exact for any reference.
+      const bool move = tmax > m_run + kLazy;
+      const float m_new = move ? tmax : m_run;
+      const float alpha = move ? fast_exp2(m_run - m_new) : 1.f;  // 0 when m_run is -inf
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      float pr[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pr[j] = fast_exp2(x[j] - m_use);
+      m_run = m_new;
+      l_run = l_run * alpha + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < kDTiles; ++i) oacc[i] *= alpha;
+      }
+      u32x2 pop, pop2 = {0u, 0u};
+      {
+        uint32_t s0_ = 0, s1_ = 0;
+        pop = u32x2{terms2(pr[0], pr[1], s0_), terms2(pr[2], pr[3], s1_)};
+        if constexpr (kSecond) pop2 = u32x2{s0_, s1_};
+      }
+      // O^T += V^T . P^T, V^T read transposed.
+      u32x2 vop[kDTiles];
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) vop[dt] = lds_read_tr4(reinterpret_cast<const BT_LDS uint16_t*>(v_at ^ (uint32_t)(dt * 32)));
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) {
+        oacc[dt] = mfma16k16(vop[dt], pop, oacc[dt]);
+        if constexpr (kSecond) oacc[dt] = mfma16k16(vop[dt], pop2, oacc[dt]);
+      }
+      rows = next_rows;
+    }
+
+    if (s1 < t1) {  // the next sequence's queries: behind its first tile, which is on its way too
+      seek(s1);
+      load_q(win.first + win.find(s1));
+    }
+
+    // ---- the waves' parts, merged ------------------------------------------------
+    l_run = halves_sum(rows16_sum(l_run));
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) oacc[dt][j] = term_sum<GMAX>(oacc[dt][j]);
+      asm volatile("" : "+v"(oacc[dt]));  // the lane moves stay here, where every lane is active
+    }
+    float* mm = mstat;
+    float* ml = mstat + kWaves * GMAX;
+    if (col_head < G) {
+      // Every column group holds the sums: group `term` stores d-tiles term, term + kGroups, ...
+      float* dst = mlds + (wave * GMAX + col_head) * kMoStride + term * 16 + kg * 4;
+#pragma unroll
+      for (int i = 0; i < kDTiles / kGroups; ++i) {
+        float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) {
+          const floatx4 a = oacc[i * kGroups + c];
+          if (c == 0 || term == c) v = float4{a[0], a[1], a[2], a[3]};
+        }
+        *reinterpret_cast<float4*>(dst + i * kGroups * 16) = v;
+      }
+      if (kg == 0 && term == 0) {
+        mm[wave * GMAX + col_head] = m_run;
+        ml[wave * GMAX + col_head] = l_run;
+      }
+    }
+    // Orders LDS only: the next tiles' loads stay on their way.
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // The waves dealt a tile: (s0 - t0) % 8 and the following ones, as many as tiles.
+    auto merge = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      const int w0 = s0 - t0;
+      for (int item = threadIdx.x; item < G * (D / 4); item += kThreads) {
+        const int h = item / (D / 4), d = item % (D / 4) * 4;
+        float mw[NW], lw[NW];
+        float4 ow[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const int at = ((w0 + i) & (kWaves - 1)) * GMAX + h;
+          mw[i] = mm[at];
+          lw[i] = ml[at];
+          ow[i] = *reinterpret_cast<const float4*>(mlds + at * kMoStride + d);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) mx = fmaxf(mx, mw[i]);
+        float lsum = 0.f;
+        float4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const float e = fast_exp2(mw[i] - mx);
+          const float sc = lw[i] == 0.f ? 0.f : e;  // no keys; a NaN sum stays one
+          lsum += lw[i] * sc;
+          acc.x += ow[i].x * sc; acc.y += ow[i].y * sc; acc.z += ow[i].z * sc; acc.w += ow[i].w * sc;
+        }
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+        acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+        if (s0 == seq_begin && s1 == seq_end) {
+          store_out(b, h, d, acc);
+        } else {
+          const int64_t row = (int64_t)(head0 + h) * (p.runs + p.batch) + w + b;
+          *reinterpret_cast<float4*>(p.part + row * D + d) = acc;
+          if (d == 0) p.lse[row] = lsum == 0.f ? -INFINITY : fast_log2(lsum) + mx;
+        }
+      }
+    };
+    if (s1 - s0 <= 2) merge(IntConst<2>{});
+    else if (s1 - s0 <= 4) merge(IntConst<4>{});
+    else merge(IntConst<kWaves>{});
+    s0 = s1;
   }
 }
 
-template <int D>
+template <int GMAX, int D>
 hipError_t launch_dim(const PagedDecodeParams& p, hipStream_t stream) {
-  const dim3 grid(p.batch * p.heads);
-  if (p.q_bf16) hipLaunchKernelGGL((gqa_paged_kernel<D, true>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((gqa_paged_kernel<D, false>), grid, dim3(256), 0, stream, p);
+  const dim3 grid(p.runs * p.kv_heads), block(kWaves * 64);
+  if (p.q_bf16) {
+    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, false>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, true>), grid, block, 0, stream, p);
+  } else {
+    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, false>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, true>), grid, block, 0, stream, p);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
+int paged_runs(int batch, int kv_heads, int head_dim, int64_t max_tokens, int num_cus) {
+  const int64_t most = (int64_t)batch * ((max_tokens + 15) / 16);  // tiles of the largest call
+  if (batch * max_tokens * head_dim <= 32768) return 1;
+  const int per_cu = head_dim == 256 ? 1 : 2;
+  int64_t runs = (int64_t)num_cus * per_cu / kv_heads;
+  const int64_t enough = (most + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
+  if (runs > enough) runs = enough;
+  return runs < 1 ? 1 : (int)runs;
+}
+
 hipError_t launch_decode_paged(const PagedDecodeParams& p, int head_dim, hipStream_t stream) {
+  const bool small = p.group <= 4;
+  hipError_t e;
   switch (head_dim) {
-    case 64: return launch_dim<64>(p, stream);
-    case 128: return launch_dim<128>(p, stream);
-    case 256: return launch_dim<256>(p, stream);
+    case 64: e = small ? launch_dim<4, 64>(p, stream) : launch_dim<8, 64>(p, stream); break;
+    case 128: e = small ? launch_dim<4, 128>(p, stream) : launch_dim<8, 128>(p, stream); break;
+    case 256: e = small ? launch_dim<4, 256>(p, stream) : launch_dim<8, 256>(p, stream); break;
     default: return hipErrorInvalidValue;
   }
+  if (e != hipSuccess || p.runs == 1) return e;
+  CombineParams c{};
+  c.lse = p.lse;
+  c.part = p.part;
+  c.total_splits = p.runs + p.batch;
+  c.split_base = p.part_base;
+  c.split_count = p.part_count;
+  c.skip_single = 1;
+  c.out = p.out;
+  c.out_bf16 = p.out_bf16;
+  c.out_stride_seq = p.out_stride_seq;
+  return launch_decode_combine(c, head_dim, p.heads, p.batch, stream);
 }
 
 }  // namespace bt

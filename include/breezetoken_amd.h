@@ -373,7 +373,7 @@ int bt_gemv_bf16(const float* x, const void* w, int64_t ldw, int32_t K, int32_t 
  * A cache in pages: num_pages pages of page_size tokens (a power of two, 16 to
  * 1,024); element (page, token, kv_head, d) of the bf16 k or v at page *
  * stride_page + token * stride_tok + kv_head * stride_head + d, strides
- * positive multiples of 8 elements.  table (rows, pages_per_seq) int32, row
+ * multiples of 8 elements, at least head_dim.  table (rows, pages_per_seq) int32, row
  * stride table_stride, holds page ids: token t of a row lies in the page of
  * entry t / page_size at token t % page_size.  Entries past a row's last token
  * are not read; an entry outside [0, num_pages) holds no keys and takes no
@@ -389,7 +389,7 @@ int64_t bt_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads,
  * attends the first lens[b] tokens of table row b (clamped to 0 ..
  * pages_per_seq * page_size; none: zeros).  q (batch, heads, head_dim) f32 or
  * bf16, out the same shape f32 or bf16.  head_dim in {64, 128, 256}, heads /
- * kv_heads <= 8, batch <= 4,096.  A page may stand in several rows, or twice in
+ * kv_heads <= 8, batch <= 4,096, batch * max_tokens < 2^34.  A page may stand in several rows, or twice in
  * one.  `workspace` is scratch for the duration of the call on `stream`: calls
  * that may overlap need one each.  It generalises gqa_decode's split and combine
  * (breezetoken/kernels/cuda/attention.py:54-205). */
