@@ -2,10 +2,20 @@
 //   score[b, w] + logit[b, w, v] - log sum_u exp(logit[b, w, u])
 // the best `beams` of each batch item, with the beam they continue and their token.
 //
-// Candidates are ordered by their value in 64 bits, equal ones by their place
-// w * vocab + v.  A NaN logit counts as -inf, a beam without a finite logit has
-// only candidates of -inf.  A logit of +inf makes its beam's others -inf and its
-// own candidate score[b, w] less the log of the number of them.
+// A beam's candidates are ordered by their logits, equal ones by token; those of two
+// beams by their value in 64 bits, equal ones by beam.  A NaN logit counts as -inf, a
+// beam without a finite logit has only candidates of -inf.  A logit of +inf makes its
+// beam's others -inf and its own candidate the score less the log of their number.
+//
+// Bound by one read of the logits.  Every (batch item, beam) row is cut into up to 64
+// chunks, one wave each.  A wave keeps, over a chunk: per lane the maximum and the sum
+// of exponentials relative to it (each f32 exponential within 2^-22 of its value for
+// the logits that matter, batches of them added in 64 bits), and across its lanes the
+// best logits so far as sorted 64-bit keys (order of the logit, ~token).  A batch of
+// logits costs the selection one comparison with the beams-th best key unless one is
+// better; where many lanes hold better ones (a chunk's first batch), the beams-th best
+// of the lanes' maxima bounds which can matter.  A second kernel, a work-group per
+// batch item, joins the chunks of a row and then the rows.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -13,9 +23,12 @@ namespace bt {
 
 namespace {
 
-constexpr int kBeamThreads = 256;
+constexpr int kScanWaves = 4;
+constexpr int kLoads = 4;  // 16-byte loads of a lane per batch
+constexpr int kJoinWaves = 8;
+constexpr float kLog2e = 1.44269504088896340736f;
 
-// Order-preserving bits of a float (-0 as +0); NaN is taken as -inf by the caller.
+// Order-preserving bits of a float (-0 as +0), and back.
 __device__ __forceinline__ uint32_t order_bits(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -23,94 +36,245 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 __device__ __forceinline__ float from_order(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-
-template <bool BF16>
-__device__ __forceinline__ float load_logit(const void* x, int64_t i) {
-  const float f = BF16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(x)[i]) : reinterpret_cast<const float*>(x)[i];
-  return f != f ? -INFINITY : f;
+__device__ __forceinline__ uint64_t make_key(float x, int token) {
+  return (uint64_t)order_bits(x) << 32 | (uint32_t)~token;
 }
+__device__ __forceinline__ uint64_t bcast(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
-__device__ uint64_t block_max(uint64_t v, uint64_t* lds) {
-  __syncthreads();
-  lds[threadIdx.x] = v;
-  __syncthreads();
-  for (int o = kBeamThreads / 2; o; o >>= 1) {
-    if ((int)threadIdx.x < o && lds[threadIdx.x + o] > lds[threadIdx.x]) lds[threadIdx.x] = lds[threadIdx.x + o];
-    __syncthreads();
+// A wave's best keys, sorted: lane i holds the i-th (0: none).
+struct Best {
+  uint64_t key = 0;
+  __device__ __forceinline__ void insert(uint64_t k) {
+    const int at = __popcll(__builtin_amdgcn_ballot_w64(key > k));
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)key, 0x138, 0xf, 0xf, false);  // wave_shr:1
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(key >> 32), 0x138, 0xf, 0xf, false);
+    const uint64_t up = (uint64_t)hi << 32 | lo;
+    key = lane_id() < at ? key : (lane_id() == at ? k : up);
   }
-  return lds[0];
-}
-__device__ double block_sum(double v, double* lds) {
-  __syncthreads();
-  lds[threadIdx.x] = v;
-  __syncthreads();
-  for (int o = kBeamThreads / 2; o; o >>= 1) {
-    if ((int)threadIdx.x < o) lds[threadIdx.x] += lds[threadIdx.x + o];
-    __syncthreads();
+};
+
+// How many lanes hold a larger key, or the same one in a lower lane: 0 .. 63, each once.
+__device__ __forceinline__ int rank_of(uint64_t k) {
+  int n = 0;
+  for (int j = 0; j < 64; ++j) {
+    const uint64_t other = bcast(k, j);
+    n += other > k || (other == k && j < lane_id());
   }
-  return lds[0];
+  return n;
 }
 
-// Per (batch item, beam): the best `beams` tokens as (logit order, ~token), and the
-// amount to add to a logit.
+// One wave per chunk of a row.
 template <bool BF16>
-__global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamParams p) {
-  __shared__ uint64_t lds[kBeamThreads];
-  const int row = blockIdx.x, b = row / p.width, w = row % p.width;
-  const int64_t base = b * p.stride_batch + w * p.stride_beam;
-  uint64_t* best = reinterpret_cast<uint64_t*>(p.ws) + (int64_t)row * (p.beams + 2);
-  uint64_t last = ~0ull, top = 0;
-  for (int k = 0; k < p.beams; ++k) {
-    uint64_t mine = 0;  // below every key: no candidate left
-    for (int v = threadIdx.x; v < p.vocab; v += kBeamThreads) {
-      const uint64_t key = (uint64_t)order_bits(load_logit<BF16>(p.logits, base + v)) << 32 | (uint32_t)~v;
-      if (key < last && key > mine) mine = key;
+__global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p) {
+  constexpr int kVec = BF16 ? 8 : 4;
+  constexpr int kElems = kVec * kLoads;      // of a lane per batch
+  constexpr int kBatch = 64 * kElems;
+  struct __attribute__((packed, aligned(BF16 ? 2 : 4))) Loose { u32x4 v; };  // rows start at any element
+  const int lane = lane_id();
+  const int64_t chunk = (int64_t)blockIdx.x * kScanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (chunk >= (int64_t)p.batch * p.width * p.chunks) return;
+  const int row = (int)(chunk / p.chunks), c = (int)(chunk % p.chunks);
+  const char* src = reinterpret_cast<const char*>(p.logits) +
+                    (row / p.width * p.stride_batch + row % p.width * p.stride_beam) * (BF16 ? 2 : 4);
+  const int v0 = c * p.chunk_size;
+  const int v1 = v0 + p.chunk_size < p.vocab ? v0 + p.chunk_size : p.vocab;
+
+  // Logit e of a lane's batch that starts at v is that of token v + token_of(e).
+  auto token_of = [&](int e) { return e / kVec * (64 * kVec) + lane * kVec + e % kVec; };
+  auto logit = [&](const u32x4 (&raw)[kLoads], int e) -> float {
+    if constexpr (BF16) {
+      const uint32_t w = raw[e / 8][e % 8 / 2];
+      return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    } else {
+      return __uint_as_float(raw[e / 4][e % 4]);
     }
-    last = block_max(mine, lds);
-    if (k == 0) top = last;
-    if (threadIdx.x == 0) best[k] = last;
-    __syncthreads();
-  }
-  const float m = from_order((uint32_t)(top >> 32));
-  double sum = 0;
-  for (int v = threadIdx.x; v < p.vocab; v += kBeamThreads) {
-    const float x = load_logit<BF16>(p.logits, base + v);
-    sum += x == m ? 1.0 : exp((double)x - (double)m);
-  }
-  sum = block_sum(sum, reinterpret_cast<double*>(lds));
-  if (threadIdx.x == 0) {
-    reinterpret_cast<double*>(best)[p.beams] = (double)m;
-    reinterpret_cast<double*>(best)[p.beams + 1] = (double)p.scores[row] - log(sum);
-  }
-}
-
-// A candidate's value: the logit relative to the beam's largest, first.
-__device__ __forceinline__ double candidate(uint64_t key, double m, double add) {
-  const float x = from_order((uint32_t)(key >> 32));
-  const double v = (double)x == m && x != -INFINITY ? add : (double)x - m + add;
-  return v != v ? -(double)INFINITY : v;
-}
-
-__global__ __launch_bounds__(64) void beam_join_kernel(BeamParams p) {
-  const int b = blockIdx.x, lane = threadIdx.x;
-  const bool mine = lane < p.width;
-  const uint64_t* best = reinterpret_cast<const uint64_t*>(p.ws) + ((int64_t)b * p.width + (mine ? lane : 0)) * (p.beams + 2);
-  const double m = reinterpret_cast<const double*>(best)[p.beams], add = reinterpret_cast<const double*>(best)[p.beams + 1];
-  int at = 0;
-  for (int k = 0; k < p.beams; ++k) {
-    const uint64_t key = mine && at < p.beams ? best[at] : 0;
-    double v = key ? candidate(key, m, add) : -(double)INFINITY;
-    int from = key ? lane : 64;  // without a candidate behind every beam
-    for (int o = 32; o; o >>= 1) {
-      const double ov = __shfl_xor(v, o);
-      const int of = __shfl_xor(from, o);
-      if (of < 64 && (from == 64 || ov > v || (ov == v && of < from))) {
-        v = ov;
-        from = of;
+  };
+  auto load = [&](u32x4 (&raw)[kLoads], int v) {
+    if (v + kBatch <= v1) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        raw[j] = reinterpret_cast<const Loose*>(src + (int64_t)(v + token_of(j * kVec)) * (BF16 ? 2 : 4))->v;
+    } else {  // the chunk's end: -inf past it
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int t = v + token_of(j * kVec);
+        if (t + kVec <= v1) {
+          raw[j] = reinterpret_cast<const Loose*>(src + (int64_t)t * (BF16 ? 2 : 4))->v;
+        } else if constexpr (BF16) {
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = t + i < v1 ? reinterpret_cast<const uint16_t*>(src)[t + i] : 0xff80u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw[j][i] = pack2(x[2 * i], x[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw[j][i] = t + i < v1 ? reinterpret_cast<const uint32_t*>(src)[t + i] : 0xff800000u;
+        }
       }
     }
-    if (lane == from) {
-      const int64_t out = (int64_t)b * p.beams + k;
+  };
+
+  const int beams = p.beams;
+  Best best;
+  float tau = -INFINITY;
+  // Better keys of a batch into the list.
+  auto select = [&](const u32x4 (&raw)[kLoads], int v) {
+    auto key_of = [&](int e) -> uint64_t {
+      const int t = v + token_of(e);
+      return t < v1 ? make_key(fmaxf(logit(raw, e), -INFINITY), t) : 0;  // fmaxf: NaN as -inf
+    };
+    uint64_t least = bcast(best.key, beams - 1), mine = 0;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+      const uint64_t k = key_of(e);
+      mine = k > mine ? k : mine;
+    }
+    if (__popcll(__builtin_amdgcn_ballot_w64(mine > least)) >= beams) {
+      const uint64_t bound = bcast(mine, __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank_of(mine) == beams - 1)));
+      if (bound > least) least = bound - 1;
+    }
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+      const uint64_t k = key_of(e);
+      uint64_t mask = __builtin_amdgcn_ballot_w64(k > least);
+      while (mask) {
+        const int l = __builtin_ctzll(mask);
+        mask &= mask - 1;
+        best.insert(bcast(k, l));
+      }
+      const uint64_t now = bcast(best.key, beams - 1);
+      least = now > least ? now : least;
+    }
+    // Later tokens of the same logit come after: only larger ones matter from here.  (A
+    // list that is not full has seen its whole chunk: a batch holds over 64 logits.)
+    tau = from_order((uint32_t)(bcast(best.key, beams - 1) >> 32));
+  };
+
+  float m = -INFINITY;
+  double sum = 0;
+  u32x4 raw[kLoads], next[kLoads];
+  load(raw, v0);
+  for (int v = v0; v < v1; v += kBatch) {
+    if (v + kBatch < v1) load(next, v + kBatch);
+    float top = m;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) top = fmaxf(top, logit(raw, e));
+    const float use = top == -INFINITY ? 0.f : top;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2((logit(raw, e) - use) * kLog2e);
+    sum = sum * (double)fast_exp2((m - use) * kLog2e) + (double)((part[0] + part[1]) + (part[2] + part[3]));
+    m = top;
+    if (v == v0 || __builtin_amdgcn_ballot_w64(top > tau)) select(raw, v);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) raw[j] = next[j];
+  }
+  // Over the lanes: relative to the largest maximum.
+  const float top = wave_fmaxf(m);
+  if (__builtin_amdgcn_ballot_w64(sum != sum)) {  // NaN or +inf among the logits: once more, with care
+    sum = 0;
+    for (int t = v0 + lane; t < v1; t += 64) {
+      const float x = fmaxf(BF16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(src)[t]) : reinterpret_cast<const float*>(src)[t],
+                            -INFINITY);
+      sum += x == top ? 1.0 : exp((double)x - (double)top);
+    }
+  } else {
+    sum = m == -INFINITY ? 0.0 : sum * exp((double)m - (double)top);
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+
+  uint64_t* keys = reinterpret_cast<uint64_t*>(p.ws) + (int64_t)row * p.chunks * (beams + 2);
+  if (lane < beams) keys[(int64_t)lane * p.chunks + c] = best.key;  // [place][chunk]
+  double* stats = reinterpret_cast<double*>(keys + (int64_t)beams * p.chunks);
+  if (lane == 0) {
+    stats[c] = (double)top;
+    stats[p.chunks + c] = sum;
+  }
+}
+
+// The larger of two keys over lanes l and l ^ MASK, for every step of a wave-wide maximum.
+template <int MASK>
+__device__ __forceinline__ uint64_t xor_max64(uint64_t x) {
+  const uint32_t lo = (uint32_t)x, hi = (uint32_t)(x >> 32);
+  uint64_t a, b;
+  if constexpr (MASK == 16 || MASK == 32) {
+    const auto l = MASK == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = MASK == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    a = (uint64_t)h[0] << 32 | l[0];
+    b = (uint64_t)h[1] << 32 | l[1];
+  } else {
+    a = x;
+    b = (uint64_t)xor_partner_bits<MASK>(hi) << 32 | xor_partner_bits<MASK>(lo);
+  }
+  return a > b ? a : b;
+}
+__device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
+  return xor_max64<1>(xor_max64<2>(xor_max64<4>(xor_max64<8>(xor_max64<16>(xor_max64<32>(x))))));
+}
+
+__global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p) {
+  __shared__ uint64_t row_keys[kMaxBeamWidth * kMaxBeams];
+  __shared__ double row_max[kMaxBeamWidth], row_add[kMaxBeamWidth];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.x, beams = p.beams, chunks = p.chunks;
+  for (int w = wave; w < p.width; w += (int)(blockDim.x >> 6)) {
+    const uint64_t* keys = reinterpret_cast<const uint64_t*>(p.ws) + ((int64_t)b * p.width + w) * chunks * (beams + 2);
+    const double* stats = reinterpret_cast<const double*>(keys + (int64_t)beams * chunks);
+    const bool mine = lane < chunks;
+    uint64_t k = mine ? keys[lane] : 0;
+    const double m = mine ? stats[lane] : -(double)INFINITY;
+    double sum = mine ? stats[chunks + lane] : 0.0;
+    const float score = p.scores[(int64_t)b * p.width + w];
+    // The chunks' best keys sorted, then the further ones while any is better than the last taken.
+    Best best;
+    const int rank = rank_of(k);
+    best.key = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(k >> 32)) << 32 |
+               (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)k);
+    uint64_t next = mine && beams > 1 ? keys[chunks + lane] : 0;
+    for (int i = 1; i < beams; ++i) {
+      k = next;
+      next = mine && i + 1 < beams ? keys[(int64_t)(i + 1) * chunks + lane] : 0;
+      uint64_t mask = __builtin_amdgcn_ballot_w64(k > bcast(best.key, beams - 1));
+      if (!mask) break;
+      while (mask) {
+        const int l = __builtin_ctzll(mask);
+        mask &= mask - 1;
+        best.insert(bcast(k, l));
+      }
+    }
+    if (lane < beams) row_keys[w * beams + lane] = best.key;
+    double top = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
+    sum = m == top ? sum : sum * exp(m - top);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) {
+      row_max[w] = top;
+      row_add[w] = (double)score - log(sum);
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  // The rows' lists, sorted each: the best of their heads, one after the other.
+  const bool mine = lane < p.width;
+  const double top = mine ? row_max[lane] : 0.0, add = mine ? row_add[lane] : 0.0;
+  int at = 0;
+  for (int i = 0; i < beams; ++i) {
+    const uint64_t key = mine && at < beams ? row_keys[lane * beams + at] : 0;
+    const double x = (double)from_order((uint32_t)(key >> 32));
+    double v = x == top && x != -(double)INFINITY ? add : x - top + add;
+    v = v != v ? -(double)INFINITY : v + 0.0;
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t order = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
+    const uint64_t most = wave_max64(order);
+    if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(order == most))) {
+      const int64_t out = (int64_t)b * beams + i;
       p.scores_out[out] = (float)v;
       p.parent_out[out] = b * p.width + lane;
       p.token_out[out] = (int)~(uint32_t)key;
@@ -121,13 +285,32 @@ __global__ __launch_bounds__(64) void beam_join_kernel(BeamParams p) {
 
 }  // namespace
 
-int64_t beam_ws_bytes(int batch, int width, int vocab, int beams) { return (int64_t)batch * width * (beams + 2) * 8; }
+// Chunks of a row, at most 64, and their size (whole wave loads): 4,096 waves in all where
+// the rows are long enough.
+int beam_chunks(int batch, int width, int vocab, int* size) {
+  const int64_t rows = (int64_t)batch * width;
+  int64_t want = (4096 + rows - 1) / rows;
+  want = want < 64 ? want : 64;
+  const int64_t per = ((int64_t)vocab + want - 1) / want;
+  const int64_t unit = 512;
+  *size = (int)((per + unit - 1) / unit * unit);
+  return (int)(((int64_t)vocab + *size - 1) / *size);
+}
 
-hipError_t launch_beam_select(const BeamParams& p, hipStream_t stream) {
-  const dim3 rows(p.batch * p.width);
-  if (p.bf16) hipLaunchKernelGGL(beam_rows_kernel<true>, rows, dim3(kBeamThreads), 0, stream, p);
-  else hipLaunchKernelGGL(beam_rows_kernel<false>, rows, dim3(kBeamThreads), 0, stream, p);
-  hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), dim3(64), 0, stream, p);
+int64_t beam_ws_bytes(int batch, int width, int vocab, int beams) {
+  int size;
+  return (int64_t)batch * width * beam_chunks(batch, width, vocab, &size) * (beams + 2) * 8;
+}
+
+hipError_t launch_beam_select(const BeamParams& params, hipStream_t stream) {
+  BeamParams p = params;
+  p.chunks = beam_chunks(p.batch, p.width, p.vocab, &p.chunk_size);
+  const int64_t waves = (int64_t)p.batch * p.width * p.chunks;
+  const dim3 grid((unsigned)((waves + kScanWaves - 1) / kScanWaves)), block(kScanWaves * 64);
+  if (p.bf16) hipLaunchKernelGGL(beam_scan_kernel<true>, grid, block, 0, stream, p);
+  else hipLaunchKernelGGL(beam_scan_kernel<false>, grid, block, 0, stream, p);
+  const int join = p.width < kJoinWaves ? p.width : kJoinWaves;
+  hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), dim3(join * 64), 0, stream, p);
   return hipGetLastError();
 }
 

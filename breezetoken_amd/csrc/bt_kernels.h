@@ -493,6 +493,7 @@ struct BeamParams {
   int64_t stride_batch, stride_beam;
   const float* scores;  // (batch, width)
   int32_t batch, width, vocab, beams;
+  int32_t chunks, chunk_size;  // of a row: set by launch_beam_select
   void* ws;  // beam_ws_bytes()
   float* scores_out;   // (batch, beams)
   int32_t* parent_out;  // (batch, beams): batch * width + beam

@@ -269,7 +269,7 @@ int bt_beam_select(const void* logits, int32_t dtype, int64_t stride_batch, int6
   if (!logits || !scores || !scores_out || !parent_out || !token_out) return BT_EINVAL;
   if (batch < 1 || width < 1 || vocab < 1 || beams < 1 || !dtype_known(dtype)) return BT_EINVAL;
   if (stride_batch < 0 || stride_beam < 0 || (int64_t)beams > (int64_t)width * vocab) return BT_EINVAL;
-  if (width > bt::kMaxBeamWidth || beams > bt::kMaxBeams || (int64_t)batch * width > INT32_MAX / 64) return BT_ENOTSUP;
+  if (vocab > (1 << 30) || width > bt::kMaxBeamWidth || beams > bt::kMaxBeams || (int64_t)batch * width > INT32_MAX / 64) return BT_ENOTSUP;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == BT_DTYPE_BF16 ? 2 : 4)) return BT_EINVAL;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bt_beam_workspace_bytes(batch, width, vocab, beams))
     return BT_ENOSPC;

@@ -470,7 +470,7 @@ int64_t bt_beam_workspace_bytes(int32_t batch, int32_t width, int32_t vocab, int
  * Sums and comparisons are in 64 bits: a beam's candidates go by their logits,
  * equal ones by token, those of two beams by value, equal ones by beam.  A NaN
  * logit counts as -inf; candidates of -inf are chosen only when no others are
- * left.  width and beams <= 64, beams <= width * vocab.  The reference decodes
+ * left.  width and beams <= 64, beams <= width * vocab, vocab <= 2^30.  The reference decodes
  * greedily (breezetoken/model/graph.py:87-91). */
 int bt_beam_select(const void* logits, int32_t dtype, int64_t stride_batch, int64_t stride_beam,
                    const float* scores, int32_t batch, int32_t width, int32_t vocab, int32_t beams,
