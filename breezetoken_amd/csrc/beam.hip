@@ -57,14 +57,17 @@ struct Best {
   }
 };
 
-// How many lanes hold a larger key, or the same one in a lower lane: 0 .. 63, each once.
-__device__ __forceinline__ int rank_of(uint64_t k) {
-  int n = 0;
-  for (int j = 0; j < 64; ++j) {
-    const uint64_t other = bcast(k, j);
-    n += other > k || (other == k && j < lane_id());
+// A bound that at least n (1 .. 64) lanes' x reach, and few more: the n-th largest to
+// within 2^-12 of its order's range between the wave's extremes.
+__device__ __forceinline__ uint32_t nth_bound(uint32_t x, int n) {
+  uint32_t lo = ~wave_umax(~x), hi = wave_umax(x);  // `lo` is reached by all
+#pragma unroll 1
+  for (int i = 0; i < 12 && lo < hi; ++i) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    if (__popcll(__builtin_amdgcn_ballot_w64(x >= mid)) >= n) lo = mid;
+    else hi = mid - 1;
   }
-  return n;
+  return lo;
 }
 
 // One wave per chunk of a row.
@@ -121,57 +124,59 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   const int beams = p.beams;
   Best best;
   float tau = -INFINITY;
-  // Better keys of a batch into the list.
-  auto select = [&](const u32x4 (&raw)[kLoads], int v) {
-    auto key_of = [&](int e) -> uint64_t {
-      const int t = v + token_of(e);
-      return t < v1 ? make_key(fmaxf(logit(raw, e), -INFINITY), t) : 0;  // fmaxf: NaN as -inf
-    };
-    uint64_t least = bcast(best.key, beams - 1), mine = 0;
+  // Better logits of a batch, whose largest of a lane is `top`, into the list.
+  auto select = [&](const u32x4 (&raw)[kLoads], int v, float top) {
+    uint64_t least = bcast(best.key, beams - 1);
+    float bound = from_order((uint32_t)(least >> 32));
+    if (least == 0) bound = -INFINITY;
+    // Enough lanes hold better ones: only those can matter that the beams-th best lane reaches.  (A lane past
+    // the chunk's end holds -inf, and raises no bound above that.)
+    const uint64_t better = __builtin_amdgcn_ballot_w64(least == 0 || top > bound);
+    if (__popcll(better) >= beams) bound = fmaxf(bound, from_order(nth_bound(order_bits(top), beams)));
 #pragma unroll
     for (int e = 0; e < kElems; ++e) {
-      const uint64_t k = key_of(e);
-      mine = k > mine ? k : mine;
-    }
-    if (__popcll(__builtin_amdgcn_ballot_w64(mine > least)) >= beams) {
-      const uint64_t bound = bcast(mine, __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank_of(mine) == beams - 1)));
-      if (bound > least) least = bound - 1;
-    }
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      const uint64_t k = key_of(e);
-      uint64_t mask = __builtin_amdgcn_ballot_w64(k > least);
-      while (mask) {
-        const int l = __builtin_ctzll(mask);
-        mask &= mask - 1;
-        best.insert(bcast(k, l));
+      const float x = logit(raw, e);
+      if (__builtin_amdgcn_ballot_w64(!(x < bound))) {  // NaN among them: it counts as -inf
+        const int t = v + token_of(e);
+        const uint64_t k = t < v1 ? make_key(fmaxf(x, -INFINITY), t) : 0;
+        uint64_t mask = __builtin_amdgcn_ballot_w64(!(x < bound) && k > least);
+        if (mask) {
+          do {
+            const int l = __builtin_ctzll(mask);
+            mask &= mask - 1;
+            best.insert(bcast(k, l));
+          } while (mask);
+          least = bcast(best.key, beams - 1);
+        }
       }
-      const uint64_t now = bcast(best.key, beams - 1);
-      least = now > least ? now : least;
     }
     // Later tokens of the same logit come after: only larger ones matter from here.  (A
     // list that is not full has seen its whole chunk: a batch holds over 64 logits.)
-    tau = from_order((uint32_t)(bcast(best.key, beams - 1) >> 32));
+    tau = from_order((uint32_t)(least >> 32));
   };
 
   float m = -INFINITY;
   double sum = 0;
-  u32x4 raw[kLoads], next[kLoads];
+  u32x4 raw[kLoads], next[kLoads], after[kLoads];
   load(raw, v0);
+  if (v0 + kBatch < v1) load(next, v0 + kBatch);
   for (int v = v0; v < v1; v += kBatch) {
-    if (v + kBatch < v1) load(next, v + kBatch);
-    float top = m;
+    if (v + 2 * kBatch < v1) load(after, v + 2 * kBatch);
+    float most = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) top = fmaxf(top, logit(raw, e));
-    const float use = top == -INFINITY ? 0.f : top;
+    for (int e = 0; e < kElems; ++e) most = fmaxf(most, logit(raw, e));
+    const float top = fmaxf(m, most), use = top == -INFINITY ? 0.f : top;
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2((logit(raw, e) - use) * kLog2e);
     sum = sum * (double)fast_exp2((m - use) * kLog2e) + (double)((part[0] + part[1]) + (part[2] + part[3]));
     m = top;
-    if (v == v0 || __builtin_amdgcn_ballot_w64(top > tau)) select(raw, v);
+    if (v == v0 || __builtin_amdgcn_ballot_w64(most > tau)) select(raw, v, most);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) raw[j] = next[j];
+    for (int j = 0; j < kLoads; ++j) {
+      raw[j] = next[j];
+      next[j] = after[j];
+    }
   }
   // Over the lanes: relative to the largest maximum.
   const float top = wave_fmaxf(m);
@@ -197,28 +202,9 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   }
 }
 
-// The larger of two keys over lanes l and l ^ MASK, for every step of a wave-wide maximum.
-template <int MASK>
-__device__ __forceinline__ uint64_t xor_max64(uint64_t x) {
-  const uint32_t lo = (uint32_t)x, hi = (uint32_t)(x >> 32);
-  uint64_t a, b;
-  if constexpr (MASK == 16 || MASK == 32) {
-    const auto l = MASK == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
-    const auto h = MASK == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
-    a = (uint64_t)h[0] << 32 | l[0];
-    b = (uint64_t)h[1] << 32 | l[1];
-  } else {
-    a = x;
-    b = (uint64_t)xor_partner_bits<MASK>(hi) << 32 | xor_partner_bits<MASK>(lo);
-  }
-  return a > b ? a : b;
-}
-__device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
-  return xor_max64<1>(xor_max64<2>(xor_max64<4>(xor_max64<8>(xor_max64<16>(xor_max64<32>(x))))));
-}
-
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p) {
   __shared__ uint64_t row_keys[kMaxBeamWidth * kMaxBeams];
+  __shared__ uint64_t order[kMaxBeamWidth * kMaxBeams];
   __shared__ double row_max[kMaxBeamWidth], row_add[kMaxBeamWidth];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x, beams = p.beams, chunks = p.chunks;
@@ -226,25 +212,31 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     const uint64_t* keys = reinterpret_cast<const uint64_t*>(p.ws) + ((int64_t)b * p.width + w) * chunks * (beams + 2);
     const double* stats = reinterpret_cast<const double*>(keys + (int64_t)beams * chunks);
     const bool mine = lane < chunks;
-    uint64_t k = mine ? keys[lane] : 0;
     const double m = mine ? stats[lane] : -(double)INFINITY;
     double sum = mine ? stats[chunks + lane] : 0.0;
     const float score = p.scores[(int64_t)b * p.width + w];
-    // The chunks' best keys sorted, then the further ones while any is better than the last taken.
+    // The chunks' lists are sorted: their first keys, then the second ones, ... while any is better
+    // than the last taken.  Four places are on their way at a time.
     Best best;
-    const int rank = rank_of(k);
-    best.key = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(k >> 32)) << 32 |
-               (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)k);
-    uint64_t next = mine && beams > 1 ? keys[chunks + lane] : 0;
-    for (int i = 1; i < beams; ++i) {
-      k = next;
-      next = mine && i + 1 < beams ? keys[(int64_t)(i + 1) * chunks + lane] : 0;
-      uint64_t mask = __builtin_amdgcn_ballot_w64(k > bcast(best.key, beams - 1));
-      if (!mask) break;
-      while (mask) {
-        const int l = __builtin_ctzll(mask);
-        mask &= mask - 1;
-        best.insert(bcast(k, l));
+    bool more = true;
+    for (int i0 = 0; i0 < beams && more; i0 += 4) {
+      uint64_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = mine && i0 + i < beams ? keys[(int64_t)(i0 + i) * chunks + lane] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint64_t least = bcast(best.key, beams - 1);
+        uint64_t mask = __builtin_amdgcn_ballot_w64(k[i] > least);
+        if (__popcll(mask) > beams) {  // none below the beams-th largest matters
+          const uint32_t bound = nth_bound((uint32_t)(k[i] >> 32), beams);
+          mask = __builtin_amdgcn_ballot_w64(k[i] > least && (uint32_t)(k[i] >> 32) >= bound);
+        }
+        more = mask != 0;
+        while (mask) {
+          const int l = __builtin_ctzll(mask);
+          mask &= mask - 1;
+          best.insert(bcast(k[i], l));
+        }
       }
     }
     if (lane < beams) row_keys[w * beams + lane] = best.key;
@@ -260,25 +252,41 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     }
   }
   __syncthreads();
-  if (wave != 0) return;
-  // The rows' lists, sorted each: the best of their heads, one after the other.
-  const bool mine = lane < p.width;
-  const double top = mine ? row_max[lane] : 0.0, add = mine ? row_add[lane] : 0.0;
-  int at = 0;
-  for (int i = 0; i < beams; ++i) {
-    const uint64_t key = mine && at < beams ? row_keys[lane * beams + at] : 0;
+  // Every row's candidates by their value, then each one's rank: how many of the other rows' sorted
+  // lists come before it.
+  const int all = p.width * beams;
+  for (int i = threadIdx.x; i < all; i += blockDim.x) {
+    const uint64_t key = row_keys[i];
+    const double top = row_max[i / beams], add = row_add[i / beams];
     const double x = (double)from_order((uint32_t)(key >> 32));
     double v = x == top && x != -(double)INFINITY ? add : x - top + add;
     v = v != v ? -(double)INFINITY : v + 0.0;
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint64_t order = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
-    const uint64_t most = wave_max64(order);
-    if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(order == most))) {
-      const int64_t out = (int64_t)b * beams + i;
-      p.scores_out[out] = (float)v;
-      p.parent_out[out] = b * p.width + lane;
-      p.token_out[out] = (int)~(uint32_t)key;
-      ++at;
+    order[i] = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;  // 0: no candidate, behind every other
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < all; i += blockDim.x) {
+    const uint64_t mine = order[i];
+    const int w = i / beams;
+    if (mine == 0) continue;
+    int rank = i - w * beams;
+    for (int o = 0; o < p.width; ++o) {
+      if (o == w) continue;
+      const uint64_t least = o < w ? mine : mine + 1;  // equal ones of lower rows come before
+      int lo = 0, hi = beams;  // places of row o that come before: [0, lo), from hi on none
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (order[o * beams + mid] >= least) lo = mid + 1;
+        else hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < beams) {
+      const int64_t out = (int64_t)b * beams + rank;
+      const uint64_t u = mine >> 63 ? mine & ~(1ull << 63) : ~mine;
+      p.scores_out[out] = (float)__builtin_bit_cast(double, u);
+      p.parent_out[out] = b * p.width + w;
+      p.token_out[out] = (int)~(uint32_t)row_keys[i];
     }
   }
 }
