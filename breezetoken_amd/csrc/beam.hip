@@ -24,7 +24,8 @@ namespace bt {
 namespace {
 
 constexpr int kScanWaves = 4;
-constexpr int kLoads = 4;  // 16-byte loads of a lane per batch
+constexpr int kLoads = 4;    // 16-byte loads of a lane per batch
+constexpr int kBatches = 4;  // batches held in registers
 constexpr int kJoinWaves = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   const int beams = p.beams;
   Best best;
   float tau = -INFINITY;
-  // Better logits of a batch, whose largest of a lane is `top`, into the list.
-  auto select = [&](const u32x4 (&raw)[kLoads], int v, float top) {
+  // Better logits of the batches held, whose largest of a lane is `top`, into the list.
+  auto select = [&](const u32x4 (&raw)[kBatches][kLoads], int v, float top) {
     uint64_t least = bcast(best.key, beams - 1);
     float bound = from_order((uint32_t)(least >> 32));
     if (least == 0) bound = -INFINITY;
@@ -134,49 +135,59 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
     const uint64_t better = __builtin_amdgcn_ballot_w64(least == 0 || top > bound);
     if (__popcll(better) >= beams) bound = fmaxf(bound, from_order(nth_bound(order_bits(top), beams)));
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      const float x = logit(raw, e);
-      if (__builtin_amdgcn_ballot_w64(!(x < bound))) {  // NaN among them: it counts as -inf
-        const int t = v + token_of(e);
-        const uint64_t k = t < v1 ? make_key(fmaxf(x, -INFINITY), t) : 0;
-        uint64_t mask = __builtin_amdgcn_ballot_w64(!(x < bound) && k > least);
-        if (mask) {
-          do {
-            const int l = __builtin_ctzll(mask);
-            mask &= mask - 1;
-            best.insert(bcast(k, l));
-          } while (mask);
-          least = bcast(best.key, beams - 1);
+    for (int i = 0; i < kBatches; ++i) {
+      if (v + i * kBatch >= v1) break;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const float x = logit(raw[i], e);
+        if (__builtin_amdgcn_ballot_w64(!(x < bound))) {  // NaN among them: it counts as -inf
+          const int t = v + i * kBatch + token_of(e);
+          const uint64_t k = t < v1 ? make_key(fmaxf(x, -INFINITY), t) : 0;
+          uint64_t mask = __builtin_amdgcn_ballot_w64(!(x < bound) && k > least);
+          if (mask) {
+            do {
+              const int l = __builtin_ctzll(mask);
+              mask &= mask - 1;
+              best.insert(bcast(k, l));
+            } while (mask);
+            least = bcast(best.key, beams - 1);
+          }
         }
       }
     }
     // Later tokens of the same logit come after: only larger ones matter from here.  (A
-    // list that is not full has seen its whole chunk: a batch holds over 64 logits.)
+    // list that is not full has seen its whole chunk: a full batch holds over 64 logits.)
     tau = from_order((uint32_t)(least >> 32));
   };
 
   float m = -INFINITY;
   double sum = 0;
-  u32x4 raw[kLoads], next[kLoads], after[kLoads];
-  load(raw, v0);
-  if (v0 + kBatch < v1) load(next, v0 + kBatch);
-  for (int v = v0; v < v1; v += kBatch) {
-    if (v + 2 * kBatch < v1) load(after, v + 2 * kBatch);
+  // All of a chunk of up to kBatches batches is held at once: every load is on its way before the first is used,
+  // the exponentials have one reference, and the selection's bound comes from all of them.
+  u32x4 raw[kBatches][kLoads];
+  for (int v = v0; v < v1; v += kBatches * kBatch) {
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i)
+      if (v + i * kBatch < v1) load(raw[i], v + i * kBatch);
     float most = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) most = fmaxf(most, logit(raw, e));
-    const float top = fmaxf(m, most), use = top == -INFINITY ? 0.f : top;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kBatches; ++i) {
+      if (v + i * kBatch >= v1) break;
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2((logit(raw, e) - use) * kLog2e);
-    sum = sum * (double)fast_exp2((m - use) * kLog2e) + (double)((part[0] + part[1]) + (part[2] + part[3]));
-    m = top;
-    if (v == v0 || __builtin_amdgcn_ballot_w64(most > tau)) select(raw, v, most);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      raw[j] = next[j];
-      next[j] = after[j];
+      for (int e = 0; e < kElems; ++e) most = fmaxf(most, logit(raw[i], e));
     }
+    const float top = fmaxf(m, most), use = top == -INFINITY ? 0.f : top;
+    sum *= (double)fast_exp2((m - use) * kLog2e);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      if (v + i * kBatch >= v1) break;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2((logit(raw[i], e) - use) * kLog2e);
+      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+    }
+    if (v == v0 || __builtin_amdgcn_ballot_w64(most > tau)) select(raw, v, most);
   }
   // Over the lanes: relative to the largest maximum.
   const float top = wave_fmaxf(m);
