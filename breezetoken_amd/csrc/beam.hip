@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kScanWaves = 4;
 constexpr int kLoads = 4;    // 16-byte loads of a lane per batch
-constexpr int kBatches = 4;  // batches held in registers
 constexpr int kJoinWaves = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -58,6 +57,26 @@ struct Best {
   }
 };
 
+// Sum over the wave in 64 bits, in the same order on every run, without an LDS round trip.
+template <int MASK>
+__device__ __forceinline__ double xor_add64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+  uint64_t a = u, b;
+  if constexpr (MASK == 16 || MASK == 32) {
+    const auto l = MASK == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = MASK == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    a = (uint64_t)h[0] << 32 | l[0];
+    b = (uint64_t)h[1] << 32 | l[1];
+  } else {
+    b = (uint64_t)xor_partner_bits<MASK>(hi) << 32 | xor_partner_bits<MASK>(lo);
+  }
+  return __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b);
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+  return xor_add64<1>(xor_add64<2>(xor_add64<4>(xor_add64<8>(xor_add64<16>(xor_add64<32>(x))))));
+}
+
 // A bound that at least n (1 .. 64) lanes' x reach, and few more: the n-th largest to
 // within 2^-12 of its order's range between the wave's extremes.
 __device__ __forceinline__ uint32_t nth_bound(uint32_t x, int n) {
@@ -77,6 +96,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   constexpr int kVec = BF16 ? 8 : 4;
   constexpr int kElems = kVec * kLoads;      // of a lane per batch
   constexpr int kBatch = 64 * kElems;
+  constexpr int kBatches = BF16 ? 2 : 4;  // held in registers: 4,096 logits
   struct __attribute__((packed, aligned(BF16 ? 2 : 4))) Loose { u32x4 v; };  // rows start at any element
   const int lane = lane_id();
   const int64_t chunk = (int64_t)blockIdx.x * kScanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -201,8 +221,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   } else {
     sum = m == -INFINITY ? 0.0 : sum * exp((double)m - (double)top);
   }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  sum = wave_sum64(sum);
 
   uint64_t* keys = reinterpret_cast<uint64_t*>(p.ws) + (int64_t)row * p.chunks * (beams + 2);
   if (lane < beams) keys[(int64_t)lane * p.chunks + c] = best.key;  // [place][chunk]
@@ -216,6 +235,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p) {
   __shared__ uint64_t row_keys[kMaxBeamWidth * kMaxBeams];
   __shared__ uint64_t order[kMaxBeamWidth * kMaxBeams];
+  __shared__ int ranks[kMaxBeamWidth * kMaxBeams];
   __shared__ double row_max[kMaxBeamWidth], row_add[kMaxBeamWidth];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x, beams = p.beams, chunks = p.chunks;
@@ -251,12 +271,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
       }
     }
     if (lane < beams) row_keys[w * beams + lane] = best.key;
-    double top = m;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
-    sum = m == top ? sum : sum * exp(m - top);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    const double top = (double)wave_fmaxf((float)m);
+    sum = wave_sum64(m == top ? sum : sum * exp(m - top));
     if (lane == 0) {
       row_max[w] = top;
       row_add[w] = (double)score - log(sum);
@@ -274,29 +290,31 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     v = v != v ? -(double)INFINITY : v + 0.0;
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     order[i] = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;  // 0: no candidate, behind every other
+    ranks[i] = i % beams;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < all * p.width; i += blockDim.x) {
+    const int c = i / p.width, o = i % p.width, w = c / beams;
+    const uint64_t mine = order[c];
+    if (mine == 0 || o == w) continue;
+    const uint64_t least = o < w ? mine : mine + 1;  // equal ones of lower rows come before
+    int lo = 0, hi = beams;  // places of row o that come before: [0, lo), from hi on none
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (order[o * beams + mid] >= least) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo) atomicAdd(ranks + c, lo);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const uint64_t mine = order[i];
-    const int w = i / beams;
-    if (mine == 0) continue;
-    int rank = i - w * beams;
-    for (int o = 0; o < p.width; ++o) {
-      if (o == w) continue;
-      const uint64_t least = o < w ? mine : mine + 1;  // equal ones of lower rows come before
-      int lo = 0, hi = beams;  // places of row o that come before: [0, lo), from hi on none
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (order[o * beams + mid] >= least) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank < beams) {
+    const int rank = ranks[i];
+    if (mine && rank < beams) {
       const int64_t out = (int64_t)b * beams + rank;
       const uint64_t u = mine >> 63 ? mine & ~(1ull << 63) : ~mine;
       p.scores_out[out] = (float)__builtin_bit_cast(double, u);
-      p.parent_out[out] = b * p.width + w;
+      p.parent_out[out] = b * p.width + i / beams;
       p.token_out[out] = (int)~(uint32_t)row_keys[i];
     }
   }
