@@ -478,12 +478,8 @@ struct PageOpParams {
   int32_t* where;      // compact: (num_pages,) new place of each page, -1: free
   int32_t* ws;         // page_ws_ints() values
 };
-// Workspace: a count per page, the free pages (compact: holes, then movers), and
-// the copies: their number, then {from, to, tokens} each.
-inline int64_t page_ws_ints(int64_t num_pages, int64_t rows_out) {
-  const int64_t copies = num_pages > rows_out ? num_pages : rows_out;
-  return 2 * num_pages + 4 + 4 * copies;
-}
+// Workspace: the copies, the rows, holders of each page, and free pages.
+int64_t page_ws_ints(int64_t num_pages, int64_t rows_out);
 hipError_t launch_fork_pages(const PageOpParams& p, hipStream_t stream);
 hipError_t launch_compact_pages(const PageOpParams& p, hipStream_t stream);
 

@@ -204,7 +204,7 @@ static int page_params(bt::PageOpParams& p, void* pages, int64_t plane_stride, i
   if (planes > 1 && plane_stride / num_pages < page_stride && page_stride / planes < plane_stride) return BT_EINVAL;
   if (rows < 0 || rows_out < 0 || pages_per_seq < 1 || num_keep < 0 || (num_keep && !keep)) return BT_EINVAL;
   if ((rows && (!table || !lens)) || (rows_out && !table_out) || (table_out && table_out == table)) return BT_EINVAL;
-  if ((int64_t)pages_per_seq * page_size > INT32_MAX) return BT_ENOTSUP;
+  if ((int64_t)pages_per_seq * page_size > INT32_MAX - bt::kMaxPageSize) return BT_ENOTSUP;
   if (planes > 65535 || (int64_t)rows_out * pages_per_seq + num_keep > INT32_MAX) return BT_ENOTSUP;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bt_pages_workspace_bytes(num_pages, rows_out))
     return BT_ENOSPC;

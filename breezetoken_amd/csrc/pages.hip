@@ -3,6 +3,14 @@
 // held while a row's first ceil(len / page_size) table entries, or `keep`, name
 // it, so an ended or replaced row frees its pages by itself.  Free pages are
 // given lowest first, in row order, so the result is the same on every run.
+//
+// A plan (who holds each page, which pages go where) and the copies it asks for.
+// The copies are bound by memory.  The plan is a chain of short steps over little
+// data, bound by latency and launches: up to kSmallPages pages, kSmallRows rows
+// and kSmallCells table entries one work-group makes all of it, holders as two
+// bits of each page in LDS (held; held twice), rows in LDS, counts by prefix sums
+// over its threads.  Larger caches count holders in memory with the whole chip;
+// the steps between stay with one work-group.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -10,196 +18,381 @@ namespace bt {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kThreads = 1024;
+constexpr int kSmallPages = 1 << 18, kSmallRows = 2048, kSmallCells = 1 << 16;
 
-__device__ __forceinline__ int row_len(const PageOpParams& p, int row) {
-  if (row < 0 || row >= p.rows) return 0;
-  const int64_t cap = (int64_t)p.pages_per_seq * p.page_size;
-  const int64_t n = p.lens[row];
-  return (int)(n < 0 ? 0 : (n > cap ? cap : n));
+// A row of the result: where it comes from, its tokens, the entries it will have,
+// and the rank among the pages given of its first one.
+struct Row {
+  int from, n, need, at;  // from: its sign bit is set where the last page is copied
+};
+
+__device__ __forceinline__ int pages_of(const PageOpParams& p, int tokens) { return (tokens + p.page_size - 1) / p.page_size; }
+
+// The row that new row r continues, its tokens, and (fork) the entries needed; `over`: entries the table lacks.
+__device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over) {
+  const int from = p.parent ? p.parent[r] : r;
+  const int cap = p.pages_per_seq * p.page_size;
+  Row row{0, 0, 0, 0};
+  if (from >= 0 && from < p.rows) {
+    const int n = p.lens[from];
+    row.from = from;
+    row.n = n < 0 ? 0 : (n > cap ? cap : n);
+  }
+  const int add = p.add && p.add[r] > 0 ? p.add[r] : 0;
+  const int64_t want = ((int64_t)row.n + add + p.page_size - 1) / p.page_size;
+  row.need = (int)(want < p.pages_per_seq ? want : p.pages_per_seq);
+  over = (int)(want - row.need);
+  // Rows without new tokens write nowhere: marked by need = -1 - need.
+  if (add == 0) row.need = -1 - row.need;
+  return row;
 }
-__device__ __forceinline__ int parent_of(const PageOpParams& p, int i) { return p.parent ? p.parent[i] : i; }
+// A live entry of a row, -1 outside the cache.
+__device__ __forceinline__ int read_entry(const PageOpParams& p, const Row& row, int c) {
+  const int id = p.table[(int64_t)(row.from & 0x7fffffff) * p.pages_per_seq + c];
+  return id >= 0 && id < p.num_pages ? id : -1;
+}
+
+// Exclusive sum of v over the work-group's threads, and the total.
+__device__ __forceinline__ int block_scan(int v, int& total, int* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the sums of the scan before are read
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int s = lane < kThreads / 64 ? lds[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < kThreads / 64; o <<= 1) {
+    const int y = __shfl_up(s, o);
+    if (lane >= o) s += y;
+  }
+  total = __builtin_amdgcn_readlane(s, kThreads / 64 - 1);
+  const int before = __shfl(s, wave > 0 ? wave - 1 : 0);
+  return x - v + (wave > 0 ? before : 0);
+}
+
+// Holders of the pages, 0, 1 or more: bits in LDS, or counts in memory.
+template <bool SMALL>
+struct Holders {
+  uint32_t* once;
+  uint32_t* twice;
+  const int* count;
+  __device__ __forceinline__ void mark(int id) {
+    const uint32_t bit = 1u << (id & 31);
+    if (atomicOr(once + (id >> 5), bit) & bit) atomicOr(twice + (id >> 5), bit);
+  }
+  __device__ __forceinline__ bool held(int id) const {
+    if constexpr (SMALL) return once[id >> 5] >> (id & 31) & 1;
+    else return count[id] != 0;
+  }
+  __device__ __forceinline__ bool shared(int id) const {
+    if constexpr (SMALL) return twice[id >> 5] >> (id & 31) & 1;
+    else return count[id] > 1;
+  }
+};
+
+// Rows, live entries and holders of a small cache, by one work-group.
+__device__ __forceinline__ void small_holders(const PageOpParams& p, Holders<true>& h, Row* rows, int& over_sum) {
+  const int t = threadIdx.x;
+  for (int i = t; i < (p.num_pages + 31) / 32; i += kThreads) h.once[i] = h.twice[i] = 0;
+  over_sum = 0;
+  for (int r = t; r < p.rows_out; r += kThreads) {
+    int over;
+    rows[r] = read_row(p, r, over);
+    over_sum += over;
+    if (p.lens_out) p.lens_out[r] = rows[r].n;
+  }
+  __syncthreads();
+  const int cells = p.rows_out * p.pages_per_seq;
+  for (int i = t; i < cells; i += kThreads) {
+    const int r = i / p.pages_per_seq, c = i % p.pages_per_seq;
+    const Row row = rows[r];
+    const int id = c < pages_of(p, row.n) ? read_entry(p, row, c) : -1;
+    p.table_out[i] = id;
+    if (id >= 0) h.mark(id);
+  }
+  for (int i = t; i < p.num_keep; i += kThreads) {
+    const int id = p.keep[i];
+    if (id >= 0 && id < p.num_pages) h.mark(id);
+  }
+  __syncthreads();
+}
+
+// The same for a large one, over the whole chip; rows in the workspace.
+struct Layout {
+  int* count;   // (num_pages)
+  int* list;    // (num_pages) free pages; compact: holes
+  int* copies;  // {number}, then {from, to, tokens, -} each
+  Row* rows;    // (rows_out)
+};
+__host__ __device__ __forceinline__ Layout layout_of(const PageOpParams& p) {
+  Layout l;
+  const int64_t most = p.num_pages > p.rows_out ? p.num_pages : p.rows_out;
+  l.copies = p.ws;
+  l.rows = reinterpret_cast<Row*>(p.ws + 4 + 4 * most);
+  l.count = p.ws + 4 + 4 * most + 4 * (int64_t)p.rows_out;
+  l.list = l.count + p.num_pages;
+  return l;
+}
 
 __global__ void pages_clear_kernel(PageOpParams p) {
+  const Layout l = layout_of(p);
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < p.num_pages) p.ws[i] = 0;
+  if (i < p.num_pages) l.count[i] = 0;
 }
 
-// Holders of every page, over the new rows' live entries and `keep`.
 __global__ void pages_count_kernel(PageOpParams p) {
+  const Layout l = layout_of(p);
   const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   int id = -1;
   if (i < cells) {
     const int r = (int)(i / p.pages_per_seq), c = (int)(i % p.pages_per_seq);
-    const int from = parent_of(p, r), n = row_len(p, from);
-    if (c < (n + p.page_size - 1) / p.page_size) {
-      id = p.table[(int64_t)from * p.pages_per_seq + c];
-      if (id < 0 || id >= p.num_pages) id = -1;
-    }
+    int over;
+    const Row row = read_row(p, r, over);
+    if (c < pages_of(p, row.n)) id = read_entry(p, row, c);
     p.table_out[i] = id;
-    if (c == 0 && p.lens_out) p.lens_out[r] = n;
+    if (c == 0) {
+      l.rows[r] = row;
+      if (p.lens_out) p.lens_out[r] = row.n;
+    }
   } else if (i < cells + p.num_keep) {
     id = p.keep[i - cells];
   }
-  if (id >= 0 && id < p.num_pages) atomicAdd(p.ws + id, 1);
+  if (id >= 0 && id < p.num_pages) atomicAdd(l.count + id, 1);
 }
 
-// Exclusive sum of v over the work-group's threads, and the total.
-__device__ int block_scan(int v, int& total, int* lds) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  lds[t] = v;
-  __syncthreads();
-  for (int o = 1; o < kPlanThreads; o <<= 1) {
-    const int x = t >= o ? lds[t - o] : 0;
-    __syncthreads();
-    lds[t] += x;
-    __syncthreads();
-  }
-  total = lds[kPlanThreads - 1];
-  return lds[t] - v;
+// The entry of new row r's column c among the pages given, `free_pages` of them on the list.
+__device__ __forceinline__ void give(const PageOpParams& p, const Row& row, int r, int c, const int* list, int free_pages) {
+  const int used = pages_of(p, row.n);
+  if (c < used || c >= row.need) return;
+  const int rank = row.at + (row.from < 0) + c - used;
+  p.table_out[(int64_t)r * p.pages_per_seq + c] = rank < free_pages ? list[rank] : -1;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PageOpParams p) {
-  __shared__ int lds[kPlanThreads];
-  int* held = p.ws;
-  int* list = p.ws + p.num_pages;
-  int* copies = p.ws + 2 * (int64_t)p.num_pages;
+template <bool SMALL>
+__global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
+  __shared__ uint32_t bits[SMALL ? 2 * (kSmallPages / 32) : 1];
+  __shared__ Row small_rows[SMALL ? kSmallRows : 1];
+  __shared__ int lds[kThreads / 64];
+  const Layout l = layout_of(p);
   const int t = threadIdx.x;
-  int free_pages = 0, total;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int i = base + t;
-    const int is_free = i < p.num_pages && held[i] == 0;
-    const int at = free_pages + block_scan(is_free, total, lds);
-    if (is_free) list[at] = i;
-    free_pages += total;
+  Holders<SMALL> h{bits, bits + kSmallPages / 32, l.count};
+  Row* rows = SMALL ? small_rows : l.rows;
+  int total, over = 0;
+  if constexpr (SMALL) {
+    small_holders(p, h, rows, over);
+  } else {
+    for (int r = t; r < p.rows_out; r += kThreads) {
+      int o;
+      read_row(p, r, o);
+      over += o;
+    }
   }
-  __syncthreads();
-  int given = 0, missing = 0;
-  for (int base = 0; base < p.rows_out; base += kPlanThreads) {
+  // Pages each row is given: a copy's first, then those of its new tokens.
+  int given = 0;
+  for (int base = 0; base < p.rows_out; base += kThreads) {
     const int r = base + t;
-    int n = 0, used = 0, need = 0, fork = 0, over = 0;
-    int32_t* row = p.table_out + (int64_t)r * p.pages_per_seq;
+    int mine = 0;
+    Row row{0, 0, 0, 0};
     if (r < p.rows_out) {
-      n = row_len(p, parent_of(p, r));
-      const int add = p.add && p.add[r] > 0 ? p.add[r] : 0;
-      used = (n + p.page_size - 1) / p.page_size;
-      const int64_t want = ((int64_t)n + add + p.page_size - 1) / p.page_size;
-      need = (int)(want < p.pages_per_seq ? want : p.pages_per_seq);
-      over = (int)(want - need);
-      if (add > 0 && n % p.page_size) {
-        const int last = row[used - 1];
-        fork = last >= 0 && held[last] > 1;
+      row = rows[r];
+      const int used = pages_of(p, row.n);
+      if (row.need < 0) {
+        row.need = -1 - row.need;
+      } else if (row.n % p.page_size) {
+        const int last = read_entry(p, row, used - 1);
+        if (last >= 0 && h.shared(last)) row.from |= (int)0x80000000;
       }
+      mine = row.need - used + (row.from < 0);
     }
-    const int mine = need - used + fork;
-    int at = given + block_scan(mine, total, lds);
+    row.at = given + block_scan(mine, total, lds);
+    if (r < p.rows_out) rows[r] = row;
     given += total;
-    if (fork) {
-      const int from = row[used - 1], to = at < free_pages ? list[at] : -1;
-      ++at;
-      row[used - 1] = to;
-      copies[4 + 4 * r] = from;
-      copies[4 + 4 * r + 1] = to;
-      copies[4 + 4 * r + 2] = n % p.page_size;
-    } else if (r < p.rows_out) {
-      copies[4 + 4 * r + 1] = -1;
-    }
-    for (int c = used; c < need; ++c, ++at) row[c] = at < free_pages ? list[at] : -1;
-    block_scan(over, total, lds);
-    missing += total;
   }
+  // Free pages in order, as many as are given: a thread takes a run of pages.
+  const int run = (p.num_pages + kThreads - 1) / kThreads;
+  const int64_t first = (int64_t)t * run;
+  int mine = 0;
+  for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += !h.held((int)first + i);
+  int free_pages;
+  int at = block_scan(mine, free_pages, lds);
+  for (int i = 0; i < run && first + i < p.num_pages && at < given; ++i)
+    if (!h.held((int)first + i)) l.list[at++] = (int)first + i;
+  block_scan(over, total, lds);  // also: the list and the rows are written
   if (t == 0) {
-    copies[0] = p.rows_out;
+    l.copies[0] = p.rows_out;
+    l.copies[1] = free_pages;
     p.status[0] = given < free_pages ? free_pages - given : 0;
-    p.status[1] = missing + (given > free_pages ? given - free_pages : 0);
+    p.status[1] = total + (given > free_pages ? given - free_pages : 0);
+  }
+  for (int r = t; r < p.rows_out; r += kThreads) {
+    const Row row = rows[r];
+    int* copy = l.copies + 4 + 4 * (int64_t)r;
+    copy[1] = -1;
+    if (row.from < 0) {
+      const int last = pages_of(p, row.n) - 1, to = row.at < free_pages ? l.list[row.at] : -1;
+      copy[0] = read_entry(p, row, last);
+      copy[1] = to;
+      copy[2] = row.n % p.page_size;
+      p.table_out[(int64_t)r * p.pages_per_seq + last] = to;
+    }
+  }
+  if constexpr (SMALL) {
+    const int cells = p.rows_out * p.pages_per_seq;
+    for (int i = t; i < cells; i += kThreads) {
+      const int r = i / p.pages_per_seq;
+      give(p, rows[r], r, i % p.pages_per_seq, l.list, free_pages);
+    }
   }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PageOpParams p) {
-  __shared__ int lds[kPlanThreads];
-  int* held = p.ws;
-  int* copies = p.ws + 2 * (int64_t)p.num_pages;
+__global__ void fork_give_kernel(PageOpParams p) {
+  const Layout l = layout_of(p);
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (int64_t)p.rows_out * p.pages_per_seq) return;
+  const int r = (int)(i / p.pages_per_seq);
+  give(p, l.rows[r], r, (int)(i % p.pages_per_seq), l.list, l.copies[1]);
+}
+
+template <bool SMALL>
+__global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) {
+  __shared__ uint32_t bits[SMALL ? 2 * (kSmallPages / 32) : 1];
+  __shared__ Row small_rows[SMALL ? kSmallRows : 1];
+  __shared__ int lds[kThreads / 64];
+  const Layout l = layout_of(p);
   const int t = threadIdx.x;
-  int live = 0, total;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int i = base + t;
-    block_scan(i < p.num_pages && held[i] != 0, total, lds);
-    live += total;
+  Holders<SMALL> h{bits, bits + kSmallPages / 32, l.count};
+  int over;
+  if constexpr (SMALL) small_holders(p, h, small_rows, over);
+  // A thread takes a run of pages: the live ones, then the free places below their
+  // number (holes) and the held pages at or past it (movers), as many.
+  const int run = (p.num_pages + kThreads - 1) / kThreads;
+  const int64_t first = (int64_t)t * run;
+  int mine = 0, live;
+  for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += h.held((int)first + i);
+  block_scan(mine, live, lds);
+  int holes = 0, movers = 0, total;
+  for (int i = 0; i < run && first + i < p.num_pages; ++i) {
+    const int id = (int)first + i;
+    const bool held = h.held(id);
+    holes += !held && id < live;
+    movers += held && id >= live;
   }
-  // Hole h (a free page below `live`) takes mover h (a held page at or past it).
-  int holes = 0, movers = 0;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int i = base + t;
-    const bool in = i < p.num_pages, is_held = in && held[i] != 0;
-    const int hole = in && !is_held && i < live, mover = is_held && i >= live;
-    int at = holes + block_scan(hole, total, lds);
-    holes += total;
-    if (hole) copies[4 + 4 * at + 1] = i;
-    at = movers + block_scan(mover, total, lds);
-    movers += total;
-    if (mover) {
-      copies[4 + 4 * at] = i;
-      copies[4 + 4 * at + 2] = p.page_size;
-    }
-    if (in && !mover) p.where[i] = is_held ? i : -1;
+  int hole = block_scan(holes, total, lds), mover = block_scan(movers, total, lds);
+  for (int i = 0; i < run && first + i < p.num_pages; ++i) {
+    const int id = (int)first + i;
+    const bool held = h.held(id);
+    if (held && id >= live) l.copies[4 + 4 * (int64_t)mover++] = id;
+    else p.where[id] = held ? id : -1;
+    if (!held && id < live) l.list[hole++] = id;
   }
   __syncthreads();
-  for (int m = t; m < movers; m += kPlanThreads) p.where[copies[4 + 4 * m]] = copies[4 + 4 * m + 1];
+  for (int m = t; m < total; m += kThreads) {
+    int* copy = l.copies + 4 + 4 * (int64_t)m;
+    const int to = l.list[m];
+    copy[1] = to;
+    copy[2] = p.page_size;
+    p.where[copy[0]] = to;
+  }
   if (t == 0) {
-    copies[0] = movers;
+    l.copies[0] = total;
     p.status[0] = live;
+  }
+  if constexpr (SMALL) {
+    __syncthreads();
+    const int cells = p.rows_out * p.pages_per_seq;
+    for (int i = t; i < cells; i += kThreads) {
+      const int id = p.table_out[i];
+      if (id >= 0) p.table_out[i] = p.where[id];
+    }
   }
 }
 
 __global__ void compact_table_kernel(PageOpParams p) {
-  const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= cells) return;
+  if (i >= (int64_t)p.rows_out * p.pages_per_seq) return;
   const int id = p.table_out[i];
   if (id >= 0) p.table_out[i] = p.where[id];
 }
 
-// The plan's copies: the first `tokens` tokens of page `from` to page `to`, in every plane.
-__global__ void pages_copy_kernel(PageOpParams p) {
-  const int* copies = p.ws + 2 * (int64_t)p.num_pages;
+// The plan's copies: the first `tokens` tokens of page `from` to page `to`, in every
+// plane.  No page is both copied and copied to, so their order does not matter.
+constexpr int kCopyThreads = 256, kCopyLoads = 4;
+__global__ __launch_bounds__(kCopyThreads) void pages_copy_kernel(PageOpParams p) {
+  const int* copies = layout_of(p).copies;
   const int n = copies[0];
-  const int plane = blockIdx.y;
+  const int64_t plane = (int64_t)blockIdx.y * p.plane_stride;
   for (int c = blockIdx.x; c < n; c += gridDim.x) {
-    const int from = copies[4 + 4 * c], to = copies[4 + 4 * c + 1], tokens = copies[4 + 4 * c + 2];
-    if (to < 0) continue;
-    const u32x4* src = reinterpret_cast<const u32x4*>(p.pages + plane * p.plane_stride + from * p.page_stride);
-    u32x4* dst = reinterpret_cast<u32x4*>(p.pages + plane * p.plane_stride + to * p.page_stride);
-    const int units = tokens * (p.token_elems / 8);
-    for (int u = threadIdx.x; u < units; u += blockDim.x) dst[u] = src[u];
+    const int* copy = copies + 4 + 4 * (int64_t)c;
+    if (copy[1] < 0) continue;
+    const u32x4* src = reinterpret_cast<const u32x4*>(p.pages + plane + copy[0] * p.page_stride);
+    u32x4* dst = reinterpret_cast<u32x4*>(p.pages + plane + copy[1] * p.page_stride);
+    const int units = copy[2] * (p.token_elems / 8);
+    int u = threadIdx.x;
+    for (; u + (kCopyLoads - 1) * kCopyThreads < units; u += kCopyLoads * kCopyThreads) {
+      u32x4 x[kCopyLoads];
+#pragma unroll
+      for (int i = 0; i < kCopyLoads; ++i) x[i] = src[u + i * kCopyThreads];
+#pragma unroll
+      for (int i = 0; i < kCopyLoads; ++i) dst[u + i * kCopyThreads] = x[i];
+    }
+    for (; u < units; u += kCopyThreads) dst[u] = src[u];
   }
 }
 
-hipError_t launch_count(const PageOpParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(pages_clear_kernel, dim3((p.num_pages + 255) / 256), dim3(256), 0, stream, p);
+bool is_small(const PageOpParams& p) {
+  return p.num_pages <= kSmallPages && p.rows_out <= kSmallRows &&
+         (int64_t)p.rows_out * p.pages_per_seq + p.num_keep <= kSmallCells;
+}
+
+dim3 per_cell(int64_t n) { return dim3((unsigned)((n + 255) / 256)); }
+
+void launch_count(const PageOpParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(pages_clear_kernel, per_cell(p.num_pages), dim3(256), 0, stream, p);
   const int64_t items = (int64_t)p.rows_out * p.pages_per_seq + p.num_keep;
-  if (items) hipLaunchKernelGGL(pages_count_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  if (items) hipLaunchKernelGGL(pages_count_kernel, per_cell(items), dim3(256), 0, stream, p);
+}
+
+void launch_copy(const PageOpParams& p, int most, hipStream_t stream) {
+  if (most) hipLaunchKernelGGL(pages_copy_kernel, dim3(most < 1024 ? most : 1024, p.planes), dim3(kCopyThreads), 0, stream, p);
 }
 
 }  // namespace
 
+int64_t page_ws_ints(int64_t num_pages, int64_t rows_out) {
+  const int64_t most = num_pages > rows_out ? num_pages : rows_out;
+  return 4 + 4 * most + 4 * rows_out + 2 * num_pages;
+}
+
 hipError_t launch_fork_pages(const PageOpParams& p, hipStream_t stream) {
-  hipError_t e = launch_count(p, stream);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
-  if (p.rows_out) hipLaunchKernelGGL(pages_copy_kernel, dim3(p.rows_out < 1024 ? p.rows_out : 1024, p.planes), dim3(256), 0, stream, p);
+  if (is_small(p)) {
+    hipLaunchKernelGGL(fork_plan_kernel<true>, dim3(1), dim3(kThreads), 0, stream, p);
+  } else {
+    launch_count(p, stream);
+    hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
+    const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
+    if (cells) hipLaunchKernelGGL(fork_give_kernel, per_cell(cells), dim3(256), 0, stream, p);
+  }
+  launch_copy(p, p.add ? p.rows_out : 0, stream);  // without new tokens nothing is written, so nothing copied
   return hipGetLastError();
 }
 
 hipError_t launch_compact_pages(const PageOpParams& p, hipStream_t stream) {
-  hipError_t e = launch_count(p, stream);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
-  const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
-  if (cells) hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, stream, p);
-  hipLaunchKernelGGL(pages_copy_kernel, dim3(p.num_pages < 1024 ? p.num_pages : 1024, p.planes), dim3(256), 0, stream, p);
+  if (is_small(p)) {
+    hipLaunchKernelGGL(compact_plan_kernel<true>, dim3(1), dim3(kThreads), 0, stream, p);
+  } else {
+    launch_count(p, stream);
+    hipLaunchKernelGGL(compact_plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
+    const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
+    if (cells) hipLaunchKernelGGL(compact_table_kernel, per_cell(cells), dim3(256), 0, stream, p);
+  }
+  launch_copy(p, p.num_pages, stream);
   return hipGetLastError();
 }
 
