@@ -463,7 +463,7 @@ hipError_t launch_paged_prep(const PagedPrepParams& p, int head_dim, hipStream_t
 struct PageOpParams {
   uint16_t* pages;
   int64_t plane_stride, page_stride;
-  int32_t planes, num_pages, page_size, token_elems;
+  int32_t planes, num_pages, page_size, page_shift, token_elems;  // page_size: 1 << page_shift
   const int32_t* table;  // (rows, pages_per_seq)
   const int32_t* lens;   // (rows,)
   int32_t rows, pages_per_seq;

@@ -205,7 +205,8 @@ static int page_params(bt::PageOpParams& p, void* pages, int64_t plane_stride, i
   if (rows < 0 || rows_out < 0 || pages_per_seq < 1 || num_keep < 0 || (num_keep && !keep)) return BT_EINVAL;
   if ((rows && (!table || !lens)) || (rows_out && !table_out) || (table_out && table_out == table)) return BT_EINVAL;
   if ((int64_t)pages_per_seq * page_size > INT32_MAX - bt::kMaxPageSize) return BT_ENOTSUP;
-  if (planes > 65535 || (int64_t)rows_out * pages_per_seq + num_keep > INT32_MAX) return BT_ENOTSUP;
+  if ((int64_t)planes * 1024 + (int64_t)rows_out * pages_per_seq + num_keep > INT32_MAX) return BT_ENOTSUP;
+  if ((int64_t)rows * pages_per_seq > INT32_MAX) return BT_ENOTSUP;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bt_pages_workspace_bytes(num_pages, rows_out))
     return BT_ENOSPC;
   p.pages = static_cast<uint16_t*>(pages);
@@ -214,6 +215,7 @@ static int page_params(bt::PageOpParams& p, void* pages, int64_t plane_stride, i
   p.planes = planes;
   p.num_pages = num_pages;
   p.page_size = page_size;
+  p.page_shift = log2_of(page_size);
   p.token_elems = token_elems;
   p.table = table;
   p.lens = lens;

@@ -19,6 +19,7 @@ namespace bt {
 namespace {
 
 constexpr int kThreads = 1024;
+constexpr int kAhead = 8;  // table entries a thread has on their way at a time
 constexpr int kSmallPages = 1 << 18, kSmallRows = 2048, kSmallCells = 1 << 16;
 
 // A row of the result: where it comes from, its tokens, the entries it will have,
@@ -27,7 +28,7 @@ struct Row {
   int from, n, need, at;  // from: its sign bit is set where the last page is copied
 };
 
-__device__ __forceinline__ int pages_of(const PageOpParams& p, int tokens) { return (tokens + p.page_size - 1) / p.page_size; }
+__device__ __forceinline__ int pages_of(const PageOpParams& p, int tokens) { return (tokens + p.page_size - 1) >> p.page_shift; }
 
 // The row that new row r continues, its tokens, and (fork) the entries needed; `over`: entries the table lacks.
 __device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over) {
@@ -40,7 +41,7 @@ __device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over)
     row.n = n < 0 ? 0 : (n > cap ? cap : n);
   }
   const int add = p.add && p.add[r] > 0 ? p.add[r] : 0;
-  const int64_t want = ((int64_t)row.n + add + p.page_size - 1) / p.page_size;
+  const int64_t want = ((int64_t)row.n + add + p.page_size - 1) >> p.page_shift;
   row.need = (int)(want < p.pages_per_seq ? want : p.pages_per_seq);
   over = (int)(want - row.need);
   // Rows without new tokens write nowhere: marked by need = -1 - need.
@@ -49,7 +50,7 @@ __device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over)
 }
 // A live entry of a row, -1 outside the cache.
 __device__ __forceinline__ int read_entry(const PageOpParams& p, const Row& row, int c) {
-  const int id = p.table[(int64_t)(row.from & 0x7fffffff) * p.pages_per_seq + c];
+  const int id = p.table[(row.from & 0x7fffffff) * p.pages_per_seq + c];
   return id >= 0 && id < p.num_pages ? id : -1;
 }
 
@@ -82,9 +83,14 @@ struct Holders {
   uint32_t* once;
   uint32_t* twice;
   const int* count;
-  __device__ __forceinline__ void mark(int id) {
-    const uint32_t bit = 1u << (id & 31);
-    if (atomicOr(once + (id >> 5), bit) & bit) atomicOr(twice + (id >> 5), bit);
+  template <int N>
+  __device__ __forceinline__ void mark(const int (&id)[N]) {  // those that are not negative
+    uint32_t old[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) old[j] = id[j] >= 0 ? atomicOr(once + (id[j] >> 5), 1u << (id[j] & 31)) : 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (id[j] >= 0 && old[j] >> (id[j] & 31) & 1) atomicOr(twice + (id[j] >> 5), 1u << (id[j] & 31));
   }
   __device__ __forceinline__ bool held(int id) const {
     if constexpr (SMALL) return once[id >> 5] >> (id & 31) & 1;
@@ -96,7 +102,23 @@ struct Holders {
   }
 };
 
-// Rows, live entries and holders of a small cache, by one work-group.
+// A thread's walk over the (row, column) cells t, t + kThreads, ...: one work-group does
+// all of a small cache's, so a division for each would be most of the work.
+struct Walk {
+  int r, c, dr, dc, per_row;
+  __device__ __forceinline__ explicit Walk(int columns)
+      : r((int)threadIdx.x / columns), c((int)threadIdx.x % columns), dr(kThreads / columns), dc(kThreads % columns), per_row(columns) {}
+  __device__ __forceinline__ void step() {
+    r += dr;
+    c += dc;
+    if (c >= per_row) {
+      c -= per_row;
+      ++r;
+    }
+  }
+};
+
+// Rows and holders of a small cache, by one work-group.
 __device__ __forceinline__ void small_holders(const PageOpParams& p, Holders<true>& h, Row* rows, int& over_sum) {
   const int t = threadIdx.x;
   for (int i = t; i < (p.num_pages + 31) / 32; i += kThreads) h.once[i] = h.twice[i] = 0;
@@ -109,16 +131,23 @@ __device__ __forceinline__ void small_holders(const PageOpParams& p, Holders<tru
   }
   __syncthreads();
   const int cells = p.rows_out * p.pages_per_seq;
-  for (int i = t; i < cells; i += kThreads) {
-    const int r = i / p.pages_per_seq, c = i % p.pages_per_seq;
-    const Row row = rows[r];
-    const int id = c < pages_of(p, row.n) ? read_entry(p, row, c) : -1;
-    p.table_out[i] = id;
-    if (id >= 0) h.mark(id);
+  Walk cell(p.pages_per_seq);
+  for (int i0 = t; i0 < cells; i0 += kAhead * kThreads) {
+    int id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j, cell.step()) {
+      id[j] = -1;
+      if (cell.r < p.rows_out) {
+        const Row row = rows[cell.r];
+        if (cell.c * p.page_size < row.n) id[j] = read_entry(p, row, cell.c);
+      }
+    }
+    h.mark(id);
   }
   for (int i = t; i < p.num_keep; i += kThreads) {
     const int id = p.keep[i];
-    if (id >= 0 && id < p.num_pages) h.mark(id);
+    const int one[1] = {id < p.num_pages ? id : -1};
+    h.mark(one);
   }
   __syncthreads();
 }
@@ -156,7 +185,6 @@ __global__ void pages_count_kernel(PageOpParams p) {
     int over;
     const Row row = read_row(p, r, over);
     if (c < pages_of(p, row.n)) id = read_entry(p, row, c);
-    p.table_out[i] = id;
     if (c == 0) {
       l.rows[r] = row;
       if (p.lens_out) p.lens_out[r] = row.n;
@@ -165,14 +193,6 @@ __global__ void pages_count_kernel(PageOpParams p) {
     id = p.keep[i - cells];
   }
   if (id >= 0 && id < p.num_pages) atomicAdd(l.count + id, 1);
-}
-
-// The entry of new row r's column c among the pages given, `free_pages` of them on the list.
-__device__ __forceinline__ void give(const PageOpParams& p, const Row& row, int r, int c, const int* list, int free_pages) {
-  const int used = pages_of(p, row.n);
-  if (c < used || c >= row.need) return;
-  const int rank = row.at + (row.from < 0) + c - used;
-  p.table_out[(int64_t)r * p.pages_per_seq + c] = rank < free_pages ? list[rank] : -1;
 }
 
 template <bool SMALL>
@@ -205,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
       const int used = pages_of(p, row.n);
       if (row.need < 0) {
         row.need = -1 - row.need;
-      } else if (row.n % p.page_size) {
+      } else if ((row.n & (p.page_size - 1))) {
         const int last = read_entry(p, row, used - 1);
         if (last >= 0 && h.shared(last)) row.from |= (int)0x80000000;
       }
@@ -239,25 +259,10 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
       const int last = pages_of(p, row.n) - 1, to = row.at < free_pages ? l.list[row.at] : -1;
       copy[0] = read_entry(p, row, last);
       copy[1] = to;
-      copy[2] = row.n % p.page_size;
-      p.table_out[(int64_t)r * p.pages_per_seq + last] = to;
+      copy[2] = (row.n & (p.page_size - 1));
     }
+    if constexpr (SMALL) l.rows[r] = row;
   }
-  if constexpr (SMALL) {
-    const int cells = p.rows_out * p.pages_per_seq;
-    for (int i = t; i < cells; i += kThreads) {
-      const int r = i / p.pages_per_seq;
-      give(p, rows[r], r, i % p.pages_per_seq, l.list, free_pages);
-    }
-  }
-}
-
-__global__ void fork_give_kernel(PageOpParams p) {
-  const Layout l = layout_of(p);
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (int64_t)p.rows_out * p.pages_per_seq) return;
-  const int r = (int)(i / p.pages_per_seq);
-  give(p, l.rows[r], r, (int)(i % p.pages_per_seq), l.list, l.copies[1]);
 }
 
 template <bool SMALL>
@@ -304,46 +309,60 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) 
     l.copies[0] = total;
     p.status[0] = live;
   }
-  if constexpr (SMALL) {
-    __syncthreads();
-    const int cells = p.rows_out * p.pages_per_seq;
-    for (int i = t; i < cells; i += kThreads) {
-      const int id = p.table_out[i];
-      if (id >= 0) p.table_out[i] = p.where[id];
-    }
-  }
 }
 
-__global__ void compact_table_kernel(PageOpParams p) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+// What a plan asks for, over the whole chip: the copies, and the new table's entries.
+// A copy is the first `tokens` tokens of page `from` to page `to`, in every plane; no page
+// is both copied and copied to, so their order does not matter.
+constexpr int kApplyThreads = 256, kCopyLoads = 4;
+template <bool FORK>
+__global__ __launch_bounds__(kApplyThreads) void pages_apply_kernel(PageOpParams p, int copy_groups) {
+  const Layout l = layout_of(p);
+  if ((int)blockIdx.x < copy_groups * p.planes) {
+    const int n = l.copies[0];
+    const int64_t plane = (int64_t)(blockIdx.x / copy_groups) * p.plane_stride;
+    for (int c = blockIdx.x % copy_groups; c < n; c += copy_groups) {
+      const int* copy = l.copies + 4 + 4 * (int64_t)c;
+      if (copy[1] < 0) continue;
+      const u32x4* src = reinterpret_cast<const u32x4*>(p.pages + plane + copy[0] * p.page_stride);
+      u32x4* dst = reinterpret_cast<u32x4*>(p.pages + plane + copy[1] * p.page_stride);
+      const int units = copy[2] * (p.token_elems / 8);
+      int u = threadIdx.x;
+      for (; u + (kCopyLoads - 1) * kApplyThreads < units; u += kCopyLoads * kApplyThreads) {
+        u32x4 x[kCopyLoads];
+#pragma unroll
+        for (int i = 0; i < kCopyLoads; ++i) x[i] = src[u + i * kApplyThreads];
+#pragma unroll
+        for (int i = 0; i < kCopyLoads; ++i) dst[u + i * kApplyThreads] = x[i];
+      }
+      for (; u < units; u += kApplyThreads) dst[u] = src[u];
+    }
+    return;
+  }
+  const int64_t i = (int64_t)(blockIdx.x - copy_groups * p.planes) * kApplyThreads + threadIdx.x;
   if (i >= (int64_t)p.rows_out * p.pages_per_seq) return;
-  const int id = p.table_out[i];
-  if (id >= 0) p.table_out[i] = p.where[id];
-}
-
-// The plan's copies: the first `tokens` tokens of page `from` to page `to`, in every
-// plane.  No page is both copied and copied to, so their order does not matter.
-constexpr int kCopyThreads = 256, kCopyLoads = 4;
-__global__ __launch_bounds__(kCopyThreads) void pages_copy_kernel(PageOpParams p) {
-  const int* copies = layout_of(p).copies;
-  const int n = copies[0];
-  const int64_t plane = (int64_t)blockIdx.y * p.plane_stride;
-  for (int c = blockIdx.x; c < n; c += gridDim.x) {
-    const int* copy = copies + 4 + 4 * (int64_t)c;
-    if (copy[1] < 0) continue;
-    const u32x4* src = reinterpret_cast<const u32x4*>(p.pages + plane + copy[0] * p.page_stride);
-    u32x4* dst = reinterpret_cast<u32x4*>(p.pages + plane + copy[1] * p.page_stride);
-    const int units = copy[2] * (p.token_elems / 8);
-    int u = threadIdx.x;
-    for (; u + (kCopyLoads - 1) * kCopyThreads < units; u += kCopyLoads * kCopyThreads) {
-      u32x4 x[kCopyLoads];
-#pragma unroll
-      for (int i = 0; i < kCopyLoads; ++i) x[i] = src[u + i * kCopyThreads];
-#pragma unroll
-      for (int i = 0; i < kCopyLoads; ++i) dst[u + i * kCopyThreads] = x[i];
+  const int r = (int)(i / p.pages_per_seq), c = (int)(i % p.pages_per_seq);
+  int id = -1;
+  if constexpr (FORK) {
+    const Row row = l.rows[r];
+    const int used = pages_of(p, row.n);
+    if (c == used - 1 && row.from < 0) {
+      id = l.copies[4 + 4 * (int64_t)r + 1];
+    } else if (c < used) {
+      id = read_entry(p, row, c);
+    } else if (c < row.need) {
+      const int rank = row.at + (row.from < 0) + c - used;
+      if (rank < l.copies[1]) id = l.list[rank];
     }
-    for (; u < units; u += kCopyThreads) dst[u] = src[u];
+  } else {
+    int over;
+    const Row row = read_row(p, r, over);
+    if (c < pages_of(p, row.n)) {
+      id = read_entry(p, row, c);
+      if (id >= 0) id = p.where[id];
+    }
   }
+  p.table_out[i] = id;
 }
 
 bool is_small(const PageOpParams& p) {
@@ -359,8 +378,12 @@ void launch_count(const PageOpParams& p, hipStream_t stream) {
   if (items) hipLaunchKernelGGL(pages_count_kernel, per_cell(items), dim3(256), 0, stream, p);
 }
 
-void launch_copy(const PageOpParams& p, int most, hipStream_t stream) {
-  if (most) hipLaunchKernelGGL(pages_copy_kernel, dim3(most < 1024 ? most : 1024, p.planes), dim3(kCopyThreads), 0, stream, p);
+template <bool FORK>
+void launch_apply(const PageOpParams& p, int copies, hipStream_t stream) {
+  const int groups = copies < 1024 ? copies : 1024;
+  const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
+  const int64_t grid = (int64_t)groups * p.planes + (cells + kApplyThreads - 1) / kApplyThreads;
+  if (grid) hipLaunchKernelGGL(pages_apply_kernel<FORK>, dim3((unsigned)grid), dim3(kApplyThreads), 0, stream, p, groups);
 }
 
 }  // namespace
@@ -376,10 +399,8 @@ hipError_t launch_fork_pages(const PageOpParams& p, hipStream_t stream) {
   } else {
     launch_count(p, stream);
     hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
-    const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
-    if (cells) hipLaunchKernelGGL(fork_give_kernel, per_cell(cells), dim3(256), 0, stream, p);
   }
-  launch_copy(p, p.add ? p.rows_out : 0, stream);  // without new tokens nothing is written, so nothing copied
+  launch_apply<true>(p, p.add ? p.rows_out : 0, stream);  // without new tokens nothing is written, so nothing copied
   return hipGetLastError();
 }
 
@@ -389,10 +410,8 @@ hipError_t launch_compact_pages(const PageOpParams& p, hipStream_t stream) {
   } else {
     launch_count(p, stream);
     hipLaunchKernelGGL(compact_plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
-    const int64_t cells = (int64_t)p.rows_out * p.pages_per_seq;
-    if (cells) hipLaunchKernelGGL(compact_table_kernel, per_cell(cells), dim3(256), 0, stream, p);
   }
-  launch_copy(p, p.num_pages, stream);
+  launch_apply<false>(p, p.num_pages, stream);
   return hipGetLastError();
 }
 
