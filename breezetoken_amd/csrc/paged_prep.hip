@@ -11,6 +11,12 @@
 //
 // Tokens without a slot (position or row outside the table, page id outside the
 // cache) write no key and no value.
+//
+// Bound by memory.  A wave takes kRows rows of one token for each of its row slots
+// (a row of D values lies in D / 4 lanes, 8 values a lane at D = 512): the loads of
+// all of them go out together, and the token's position, page and angles are read
+// once.  In the half layout a value's partner comes through LDS (16 bytes a lane
+// where the half is a multiple of 4), in the interleaved one it is in the lane.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -18,86 +24,213 @@ namespace bt {
 
 namespace {
 
-// One wave per (token, row): rows 0 .. H - 1 are q heads, then k heads, then v heads.
-template <int D>
-__global__ __launch_bounds__(64) void paged_prep_kernel(PagedPrepParams p) {
-  constexpr int E = D / 64;
-  __shared__ float row[D];
-  const int rows = p.heads + 2 * p.kv_heads;
-  const int t = (int)(blockIdx.x / (unsigned)rows), r = (int)(blockIdx.x % (unsigned)rows);
-  const int lane = threadIdx.x;
-  const bool is_q = r < p.heads, is_v = r >= p.heads + p.kv_heads;
+constexpr int kWaves = 4;
+constexpr int kRows = 4;
+
+enum Rope : int { kNone = 0, kHalf = 1, kHalfOdd = 2, kPairs = 3 };  // kHalfOdd: a half that is no multiple of 4
+
+struct __attribute__((packed, aligned(4))) Loose4 {  // tables need no more than a float's alignment
+  float v[4];
+};
+
+template <int D, bool XBF16, int ROPE>
+__global__ __launch_bounds__(kWaves * 64) void paged_prep_kernel(PagedPrepParams p, int groups) {
+  constexpr int E = D == 512 ? 8 : 4;  // values of a lane
+  constexpr int kLanes = D / E;        // lanes of a row
+  constexpr int kSlots = 64 / kLanes;  // rows side by side in a wave
+  __shared__ __attribute__((aligned(16))) float lds[ROPE == kHalf || ROPE == kHalfOdd ? kWaves * 64 * E : 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned id = blockIdx.x * kWaves + wave;
+  if (id >= (unsigned)p.tokens * (unsigned)groups) return;
+  const int t = (int)(id / (unsigned)groups), g = (int)(id % (unsigned)groups);
+  const int d0 = lane % kLanes * E;
+  const int k0 = p.heads, v0 = p.heads + p.kv_heads, rows = p.heads + 2 * p.kv_heads;
+  const int row0 = g * kRows * kSlots + lane / kLanes;
+  auto row_of = [&](int j) { return row0 + j * kSlots; };
+
+  // ---- the rows' values ---------------------------------------------------------
   const int step = p.gated ? 2 * D : D;
-  const int64_t src = (int64_t)t * p.x_stride + (is_q ? (int64_t)r * step : (int64_t)p.heads * step + (int64_t)(r - p.heads) * D);
-  float x[E];
+  const int64_t token = (int64_t)t * p.x_stride;
+  float x[kRows][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int64_t at = src + lane * E + e;
-    x[e] = p.x_bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.x)[at]) : reinterpret_cast<const float*>(p.x)[at];
+  for (int j = 0; j < kRows; ++j) {
+    const int r = row_of(j);
+    if (r < rows) {
+      const int64_t at = token + (r < k0 ? r * step : p.heads * step + (r - k0) * D) + d0;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        if constexpr (XBF16) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(p.x) + at + e);
+          x[j][e] = __uint_as_float(w[0] << 16);
+          x[j][e + 1] = __uint_as_float(w[0] & 0xffff0000u);
+          x[j][e + 2] = __uint_as_float(w[1] << 16);
+          x[j][e + 3] = __uint_as_float(w[1] & 0xffff0000u);
+        } else {
+          const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at + e);
+          x[j][e] = w.x;
+          x[j][e + 1] = w.y;
+          x[j][e + 2] = w.z;
+          x[j][e + 3] = w.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[j][e] = 0.f;
+    }
   }
-  const int pos = p.pos[t];
-  const float* w = is_q ? p.wq : p.wk;
-  if (!is_v && w != nullptr) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
-    ss = wave_sum(ss);
-    const float f = 1.0f / sqrtf(ss / (float)D + p.eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * f * w[lane * E + e];
-  }
-  if (!is_v && p.cos != nullptr) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) row[lane * E + e] = x[e];
-    __syncthreads();
+
+  // ---- the token's slot and angles -------------------------------------------------
+  const int pos = __builtin_amdgcn_readfirstlane(p.pos[t]);
+  const int seq = p.rows ? __builtin_amdgcn_readfirstlane(p.rows[t]) : t;
+  int page = -1;
+  if (seq >= 0 && seq < p.table_rows && pos >= 0 && pos >> p.pg.page_shift < p.pg.pages_per_seq)
+    page = __builtin_amdgcn_readfirstlane(p.pg.table[(int64_t)seq * p.pg.table_stride + (pos >> p.pg.page_shift)]);
+  const bool slot = page >= 0 && page < p.pg.num_pages;
+  const int64_t slot_at = (int64_t)page * p.pg.stride_page + (int64_t)(pos & ((1 << p.pg.page_shift) - 1)) * p.pg.stride_tok;
+  float cs[E], sn[E];  // per value (half layouts) or per pair
+  const int half = p.rope_dim >> 1;
+  const bool turned = ROPE != kNone && d0 < p.rope_dim;
+  if constexpr (ROPE != kNone) {
     const int pr = pos < 0 ? 0 : (pos >= p.rope_cap ? p.rope_cap - 1 : pos);
     const float* c = p.cos + (int64_t)pr * p.rope_dim;
     const float* s = p.sin + (int64_t)pr * p.rope_dim;
-    const int half = p.rope_dim / 2;
+    if (turned) {
+      if constexpr (ROPE == kHalf) {
+        const int i0 = d0 < half ? d0 : d0 - half;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane * E + e;
-      if (d < p.rope_dim) {
-        const bool first = p.interleaved ? (d & 1) == 0 : d < half;
-        const int i = p.interleaved ? d >> 1 : (first ? d : d - half);
-        const float other = row[p.interleaved ? d ^ 1 : (first ? d + half : d - half)];
-        x[e] = first ? x[e] * c[i] - other * s[i] : x[e] * c[i] + other * s[i];
+        for (int e = 0; e < E; e += 4) {
+          // At D = 512 a lane's second four may lie past the half, or past rope_dim.
+          const int d = d0 + e, i = E == 4 ? i0 : (d < half ? d : (d < p.rope_dim ? d - half : 0));
+          const Loose4 cc = *reinterpret_cast<const Loose4*>(c + i), ss = *reinterpret_cast<const Loose4*>(s + i);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            cs[e + q] = cc.v[q];
+            sn[e + q] = ss.v[q];
+          }
+        }
+      } else if constexpr (ROPE == kHalfOdd) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int d = d0 + e, i = d < half ? d : (d < p.rope_dim ? d - half : 0);
+          cs[e] = c[i];
+          sn[e] = s[i];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const int i = d0 + e < p.rope_dim ? (d0 + e) >> 1 : 0;
+          cs[e] = c[i];
+          sn[e] = s[i];
+        }
       }
     }
   }
-  if (is_q) {
-    const int64_t at = ((int64_t)t * p.heads + r) * D + lane * E;
+  float* part = lds + wave * 64 * E;  // this wave's: its LDS operations stay in order
+
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (p.q_out_bf16) reinterpret_cast<uint16_t*>(p.q_out)[at + e] = (uint16_t)f32_to_bf16_bits(x[e]);
-      else reinterpret_cast<float*>(p.q_out)[at + e] = x[e];
+  for (int j = 0; j < kRows; ++j) {
+    const int r = row_of(j);
+    const bool is_v = r >= v0;
+    // ---- norm --------------------------------------------------------------------
+    if (p.wq != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss = fmaf(x[j][e], x[j][e], ss);
+      ss = xor_sum<8>(xor_sum<4>(xor_sum<2>(xor_sum<1>(ss))));
+      if constexpr (kLanes >= 32) ss = rows16_sum(ss);
+      if constexpr (kLanes >= 64) ss = halves_sum(ss);
+      const float f = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+      if (!is_v) {
+        const float* w = (r < k0 ? p.wq : p.wk) + d0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          const float4 ww = *reinterpret_cast<const float4*>(w + e);
+          x[j][e] *= f * ww.x;
+          x[j][e + 1] *= f * ww.y;
+          x[j][e + 2] *= f * ww.z;
+          x[j][e + 3] *= f * ww.w;
+        }
+      }
     }
-    return;
-  }
-  const int seq = p.rows ? p.rows[t] : t;
-  if (seq < 0 || seq >= p.table_rows || pos < 0 || (pos >> p.pg.page_shift) >= p.pg.pages_per_seq) return;
-  const int page = p.pg.table[(int64_t)seq * p.pg.table_stride + (pos >> p.pg.page_shift)];
-  if (page < 0 || page >= p.pg.num_pages) return;
-  const int g = is_v ? r - p.heads - p.kv_heads : r - p.heads;
-  const int64_t at = (int64_t)page * p.pg.stride_page + (int64_t)(pos & ((1 << p.pg.page_shift) - 1)) * p.pg.stride_tok +
-                     (int64_t)g * p.pg.stride_head + lane * E;
-  uint16_t* dst = is_v ? p.v : p.k;
+    // ---- rotation ------------------------------------------------------------------
+    if constexpr (ROPE == kHalf || ROPE == kHalfOdd) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[at + e] = (uint16_t)f32_to_bf16_bits(x[e]);
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(part + lane * E + e) = float4{x[j][e], x[j][e + 1], x[j][e + 2], x[j][e + 3]};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (turned && !is_v) {
+        const float* row = part + lane / kLanes * D;
+#pragma unroll
+        for (int e = 0; e < E; e += (ROPE == kHalf ? 4 : 1)) {
+          const int d = d0 + e;
+          if (d < p.rope_dim) {
+            const bool first = d < half;
+            const float* other = row + (first ? d + half : d - half);
+            if constexpr (ROPE == kHalf) {
+              const float4 o = *reinterpret_cast<const float4*>(other);
+              const float sg = first ? -1.f : 1.f;
+              x[j][e] = x[j][e] * cs[e] + sg * o.x * sn[e];
+              x[j][e + 1] = x[j][e + 1] * cs[e + 1] + sg * o.y * sn[e + 1];
+              x[j][e + 2] = x[j][e + 2] * cs[e + 2] + sg * o.z * sn[e + 2];
+              x[j][e + 3] = x[j][e + 3] * cs[e + 3] + sg * o.w * sn[e + 3];
+            } else {
+              x[j][e] = x[j][e] * cs[e] + (first ? -*other : *other) * sn[e];
+            }
+          }
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the next row's values take the place
+    } else if constexpr (ROPE == kPairs) {
+      if (turned && !is_v) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          if (d0 + e < p.rope_dim) {
+            const float a = x[j][e], b = x[j][e + 1];
+            x[j][e] = a * cs[e] - b * sn[e];
+            x[j][e + 1] = b * cs[e] + a * sn[e];
+          }
+        }
+      }
+    }
+    // ---- out -----------------------------------------------------------------------
+    if (r >= rows) continue;
+    if (r < k0 && !p.q_out_bf16) {
+      float* dst = reinterpret_cast<float*>(p.q_out) + ((int64_t)t * p.heads + r) * D + d0;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(dst + e) = float4{x[j][e], x[j][e + 1], x[j][e + 2], x[j][e + 3]};
+    } else {
+      if (r >= k0 && !slot) continue;
+      uint16_t* dst = r < k0 ? reinterpret_cast<uint16_t*>(p.q_out) + ((int64_t)t * p.heads + r) * D
+                             : (is_v ? p.v : p.k) + slot_at + (int64_t)(r - (is_v ? v0 : k0)) * p.pg.stride_head;
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<u32x2*>(dst + d0 + e) = u32x2{f32x2_to_bf16x2_bits(x[j][e], x[j][e + 1]), f32x2_to_bf16x2_bits(x[j][e + 2], x[j][e + 3])};
+    }
+  }
+}
+
+template <int D, bool XBF16>
+hipError_t launch_dim(const PagedPrepParams& p, hipStream_t stream) {
+  constexpr int kLanes = D / (D == 512 ? 8 : 4), kPer = kRows * (64 / kLanes);
+  const int groups = (p.heads + 2 * p.kv_heads + kPer - 1) / kPer;
+  const dim3 grid((unsigned)(((int64_t)p.tokens * groups + kWaves - 1) / kWaves)), block(kWaves * 64);
+  if (!p.cos) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kNone>), grid, block, 0, stream, p, groups);
+  else if (p.interleaved) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kPairs>), grid, block, 0, stream, p, groups);
+  else if (p.rope_dim % 8 == 0) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kHalf>), grid, block, 0, stream, p, groups);
+  else hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kHalfOdd>), grid, block, 0, stream, p, groups);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_paged_prep(const PagedPrepParams& p, int head_dim, hipStream_t stream) {
-  const dim3 grid((unsigned)p.tokens * (unsigned)(p.heads + 2 * p.kv_heads));
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL(paged_prep_kernel<64>, grid, dim3(64), 0, stream, p); break;
-    case 128: hipLaunchKernelGGL(paged_prep_kernel<128>, grid, dim3(64), 0, stream, p); break;
-    case 256: hipLaunchKernelGGL(paged_prep_kernel<256>, grid, dim3(64), 0, stream, p); break;
-    case 512: hipLaunchKernelGGL(paged_prep_kernel<512>, grid, dim3(64), 0, stream, p); break;
+    case 64: return p.x_bf16 ? launch_dim<64, true>(p, stream) : launch_dim<64, false>(p, stream);
+    case 128: return p.x_bf16 ? launch_dim<128, true>(p, stream) : launch_dim<128, false>(p, stream);
+    case 256: return p.x_bf16 ? launch_dim<256, true>(p, stream) : launch_dim<256, false>(p, stream);
+    case 512: return p.x_bf16 ? launch_dim<512, true>(p, stream) : launch_dim<512, false>(p, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace bt
