@@ -12,10 +12,11 @@
 // Tokens without a slot (position or row outside the table, page id outside the
 // cache) write no key and no value.
 //
-// Bound by memory.  A wave takes kRows rows of one token for each of its row slots
-// (a row of D values lies in D / 4 lanes, 8 values a lane at D = 512): the loads of
-// all of them go out together, and the token's position, page and angles are read
-// once.  In the half layout a value's partner comes through LDS (16 bytes a lane
+// Bound by memory: 8,192 tokens of H = 8, Hkv = 2, D = 256 (f32, gated, norm) take
+// 36 us, 4.8 TB/s, what a large copy reaches.  A wave takes kRows rows of one token
+// for each of its row slots (a row of D values lies in D / 4 lanes, 8 values a lane at
+// D = 512): the loads of all of them go out together, and the token's position, page
+// and angles are read once.  In the half layout a value's partner comes through LDS (16 bytes a lane
 // where the half is a multiple of 4), in the interleaved one it is in the lane.
 #include "bt_common.h"
 #include "bt_kernels.h"
@@ -25,7 +26,11 @@ namespace bt {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kRows = 4;
+// Calls whose rows all fit the chip at once, a row slot a wave (256 CUs hold 8,192 waves), take one row a
+// slot: latency counts.  One / four rows, us a graph node, H = 32, Hkv = 8, D = 128 (24 waves a token): 24
+// tokens 3.5 / 4.3, 256 4.7 / 5.3, 512 7.5 / 6.6, 2,048 19.3 / 15.2; H = 8, Hkv = 2, D = 256 (12 waves): 24
+// tokens 3.3 / 4.1, 512 5.6 / 6.1, 1,024 8.4 / 7.8.
+constexpr int64_t kFewWaves = 8192;
 
 enum Rope : int { kNone = 0, kHalf = 1, kHalfOdd = 2, kPairs = 3 };  // kHalfOdd: a half that is no multiple of 4
 
@@ -33,7 +38,7 @@ struct __attribute__((packed, aligned(4))) Loose4 {  // tables need no more than
   float v[4];
 };
 
-template <int D, bool XBF16, int ROPE>
+template <int D, bool XBF16, int ROPE, int kRows>
 __global__ __launch_bounds__(kWaves * 64) void paged_prep_kernel(PagedPrepParams p, int groups) {
   constexpr int E = D == 512 ? 8 : 4;  // values of a lane
   constexpr int kLanes = D / E;        // lanes of a row
@@ -209,16 +214,25 @@ __global__ __launch_bounds__(kWaves * 64) void paged_prep_kernel(PagedPrepParams
   }
 }
 
+template <int D, bool XBF16, int ROPE>
+hipError_t launch_rope(const PagedPrepParams& p, hipStream_t stream) {
+  constexpr int kSlots = 64 / (D / (D == 512 ? 8 : 4));
+  const int rows = p.heads + 2 * p.kv_heads;
+  auto launch = [&](auto kernel, int per) {
+    const int groups = (rows + per - 1) / per;
+    const dim3 grid((unsigned)(((int64_t)p.tokens * groups + kWaves - 1) / kWaves));
+    hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), 0, stream, p, groups);
+    return hipGetLastError();
+  };
+  if ((int64_t)p.tokens * ((rows + kSlots - 1) / kSlots) <= kFewWaves) return launch(paged_prep_kernel<D, XBF16, ROPE, 1>, kSlots);
+  return launch(paged_prep_kernel<D, XBF16, ROPE, 4>, 4 * kSlots);
+}
+
 template <int D, bool XBF16>
 hipError_t launch_dim(const PagedPrepParams& p, hipStream_t stream) {
-  constexpr int kLanes = D / (D == 512 ? 8 : 4), kPer = kRows * (64 / kLanes);
-  const int groups = (p.heads + 2 * p.kv_heads + kPer - 1) / kPer;
-  const dim3 grid((unsigned)(((int64_t)p.tokens * groups + kWaves - 1) / kWaves)), block(kWaves * 64);
-  if (!p.cos) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kNone>), grid, block, 0, stream, p, groups);
-  else if (p.interleaved) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kPairs>), grid, block, 0, stream, p, groups);
-  else if (p.rope_dim % 8 == 0) hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kHalf>), grid, block, 0, stream, p, groups);
-  else hipLaunchKernelGGL((paged_prep_kernel<D, XBF16, kHalfOdd>), grid, block, 0, stream, p, groups);
-  return hipGetLastError();
+  if (!p.cos) return launch_rope<D, XBF16, kNone>(p, stream);
+  if (p.interleaved) return launch_rope<D, XBF16, kPairs>(p, stream);
+  return p.rope_dim % 8 == 0 ? launch_rope<D, XBF16, kHalf>(p, stream) : launch_rope<D, XBF16, kHalfOdd>(p, stream);
 }
 
 }  // namespace
