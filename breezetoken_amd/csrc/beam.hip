@@ -7,15 +7,20 @@
 // beam without a finite logit has only candidates of -inf.  A logit of +inf makes its
 // beam's others -inf and its own candidate the score less the log of their number.
 //
-// Bound by one read of the logits.  Every (batch item, beam) row is cut into up to 64
-// chunks, one wave each.  A wave keeps, over a chunk: per lane the maximum and the sum
-// of exponentials relative to it (each f32 exponential within 2^-22 of its value for
-// the logits that matter, batches of them added in 64 bits), and across its lanes the
-// best logits so far as sorted 64-bit keys (order of the logit, ~token).  A batch of
-// logits costs the selection one comparison with the beams-th best key unless one is
-// better; where many lanes hold better ones (a chunk's first batch), the beams-th best
-// of the lanes' maxima bounds which can matter.  A second kernel, a work-group per
-// batch item, joins the chunks of a row and then the rows.
+// Every (batch item, beam) row is cut into up to 64 chunks, one wave each, four
+// neighbouring chunks a work-group.  A wave holds 4,096 logits in registers at a time.
+// The work-group's lanes exchange the largest of theirs: the beams-th largest of these
+// 256 values bounds which logits can be chosen, so of 16,384 logits little more than
+// `beams` are looked at; they enter the wave's best, sorted 64-bit keys (order of the
+// logit, ~token) across its lanes.  The largest is the exponentials' reference: c, its
+// product with log2(e) rounded to a whole number, so that each is one fused
+// multiply-add x log2(e) - c, exact to 2^-24 of itself, and one v_exp, and sums of
+// any lanes, waves and chunks add after a power of two.  They are added in 32 bits by
+// sixteens, then in 64.  A second kernel, a work-group per batch item, joins the chunks
+// of a row and then the rows.
+//
+// Bound by the vector ALU, near the time of one read of the logits (bf16: unpack, max,
+// fma, exp, add each).
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -26,6 +31,7 @@ namespace {
 constexpr int kScanWaves = 4;
 constexpr int kLoads = 4;    // 16-byte loads of a lane per batch
 constexpr int kJoinWaves = 8;
+constexpr int kStats = 3;     // of a chunk, behind its keys
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Order-preserving bits of a float (-0 as +0), and back.
@@ -77,14 +83,25 @@ __device__ __forceinline__ double wave_sum64(double x) {
   return xor_add64<1>(xor_add64<2>(xor_add64<4>(xor_add64<8>(xor_add64<16>(xor_add64<32>(x))))));
 }
 
-// A bound that at least n (1 .. 64) lanes' x reach, and few more: the n-th largest to
-// within 2^-12 of its order's range between the wave's extremes.
-__device__ __forceinline__ uint32_t nth_bound(uint32_t x, int n) {
-  uint32_t lo = ~wave_umax(~x), hi = wave_umax(x);  // `lo` is reached by all
+// A bound that at least n (1 .. 64) of the wave's 64 N values reach, and few more: the
+// n-th largest to within 2^-12 of the range between the extremes.  `top`: the largest.
+template <int N>
+__device__ __forceinline__ uint32_t nth_bound(const uint32_t (&x)[N], int n, uint32_t& top) {
+  uint32_t least = x[0], most = x[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) {
+    least = x[j] < least ? x[j] : least;
+    most = x[j] > most ? x[j] : most;
+  }
+  uint32_t lo = ~wave_umax(~least), hi = wave_umax(most);  // `lo` is reached by all
+  top = hi;
 #pragma unroll 1
   for (int i = 0; i < 12 && lo < hi; ++i) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
-    if (__popcll(__builtin_amdgcn_ballot_w64(x >= mid)) >= n) lo = mid;
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) reach += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= mid));
+    if (reach >= n) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -96,16 +113,19 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   constexpr int kVec = BF16 ? 8 : 4;
   constexpr int kElems = kVec * kLoads;      // of a lane per batch
   constexpr int kBatch = 64 * kElems;
-  constexpr int kBatches = BF16 ? 2 : 4;  // held in registers: 4,096 logits
+  constexpr int kBatches = BF16 ? 2 : 4;     // held in registers: 4,096 logits
+  constexpr int kHeld = kBatches * kBatch;
+  constexpr int kGroup = 8;                  // logits of a lane tested together
+  constexpr int kGroups = kBatches * kElems / kGroup;
   struct __attribute__((packed, aligned(BF16 ? 2 : 4))) Loose { u32x4 v; };  // rows start at any element
-  const int lane = lane_id();
-  const int64_t chunk = (int64_t)blockIdx.x * kScanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (chunk >= (int64_t)p.batch * p.width * p.chunks) return;
-  const int row = (int)(chunk / p.chunks), c = (int)(chunk % p.chunks);
+  __shared__ uint32_t lane_tops[2][kScanWaves * 64];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (p.chunks + kScanWaves - 1) / kScanWaves;
+  const int row = (int)(blockIdx.x / (unsigned)groups), c = (int)(blockIdx.x % (unsigned)groups) * kScanWaves + wave;
   const char* src = reinterpret_cast<const char*>(p.logits) +
                     (row / p.width * p.stride_batch + row % p.width * p.stride_beam) * (BF16 ? 2 : 4);
-  const int v0 = c * p.chunk_size;
-  const int v1 = v0 + p.chunk_size < p.vocab ? v0 + p.chunk_size : p.vocab;
+  const int v0 = c < p.chunks ? c * p.chunk_size : p.vocab;  // a wave past the last chunk has no logits
+  const int v1 = c < p.chunks - 1 ? v0 + p.chunk_size : p.vocab;
 
   // Logit e of a lane's batch that starts at v is that of token v + token_of(e).
   auto token_of = [&](int e) { return e / kVec * (64 * kVec) + lane * kVec + e % kVec; };
@@ -144,23 +164,63 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
 
   const int beams = p.beams;
   Best best;
-  float tau = -INFINITY;
-  // Better logits of the batches held, whose largest of a lane is `top`, into the list.
-  auto select = [&](const u32x4 (&raw)[kBatches][kLoads], int v, float top) {
+  float bound = -INFINITY;  // `beams` logits of the work-group's reach it
+  float top = -INFINITY;    // the work-group's largest
+  float ref = 0.f;          // the sum's reference: 2^ref
+  double sum = 0;
+  u32x4 raw[kBatches][kLoads];
+  for (int s = 0, odd = 0; s < p.chunk_size; s += kHeld, odd ^= 1) {
+    const int v = v0 + s;
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i)
+      if (v + i * kBatch < v1) load(raw[i], v + i * kBatch);
+    float most[kGroups], mine = -INFINITY;  // fmaxf leaves NaN out
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+#pragma unroll
+      for (int g = 0; g < kElems / kGroup; ++g) {
+        float x = -INFINITY;
+        if (v + i * kBatch < v1) {
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) x = fmaxf(x, logit(raw[i], g * kGroup + e));
+        }
+        most[i * (kElems / kGroup) + g] = x;
+        mine = fmaxf(mine, x);
+      }
+    }
+    // (Two buffers: a wave that is a pass ahead writes the other one.)
+    lane_tops[odd][threadIdx.x] = order_bits(mine);
+    __syncthreads();
+    uint32_t tops[kScanWaves], highest;
+#pragma unroll
+    for (int j = 0; j < kScanWaves; ++j) tops[j] = lane_tops[odd][j * 64 + lane];
+    bound = fmaxf(bound, from_order(nth_bound(tops, beams, highest)));
+    top = fmaxf(top, from_order(highest));
+    if (v >= v1) continue;
+
+    const float now = top == -INFINITY ? 0.f : rintf(top * kLog2e);
+    if (sum != 0.0) sum *= (double)fast_exp2(ref - now);  // whole numbers, falling: exact, or past all that counts
+    ref = now;
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      if (v + i * kBatch >= v1) break;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2(fmaf(logit(raw[i], e), kLog2e, -ref));
+      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+    }
+
     uint64_t least = bcast(best.key, beams - 1);
-    float bound = from_order((uint32_t)(least >> 32));
-    if (least == 0) bound = -INFINITY;
-    // Enough lanes hold better ones: only those can matter that the beams-th best lane reaches.  (A lane past
-    // the chunk's end holds -inf, and raises no bound above that.)
-    const uint64_t better = __builtin_amdgcn_ballot_w64(least == 0 || top > bound);
-    if (__popcll(better) >= beams) bound = fmaxf(bound, from_order(nth_bound(order_bits(top), beams)));
 #pragma unroll
     for (int i = 0; i < kBatches; ++i) {
       if (v + i * kBatch >= v1) break;
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) {
-        const float x = logit(raw[i], e);
-        if (__builtin_amdgcn_ballot_w64(!(x < bound))) {  // NaN among them: it counts as -inf
+      for (int g = 0; g < kElems / kGroup; ++g) {
+        if (!__builtin_amdgcn_ballot_w64(most[i * (kElems / kGroup) + g] >= bound)) continue;
+#pragma unroll
+        for (int e = g * kGroup; e < (g + 1) * kGroup; ++e) {
+          const float x = logit(raw[i], e);
+          if (!__builtin_amdgcn_ballot_w64(!(x < bound))) continue;  // NaN counts as -inf
           const int t = v + i * kBatch + token_of(e);
           const uint64_t k = t < v1 ? make_key(fmaxf(x, -INFINITY), t) : 0;
           uint64_t mask = __builtin_amdgcn_ballot_w64(!(x < bound) && k > least);
@@ -175,60 +235,28 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
         }
       }
     }
-    // Later tokens of the same logit come after: only larger ones matter from here.  (A
-    // list that is not full has seen its whole chunk: a full batch holds over 64 logits.)
-    tau = from_order((uint32_t)(least >> 32));
-  };
-
-  float m = -INFINITY;
-  double sum = 0;
-  // All of a chunk of up to kBatches batches is held at once: every load is on its way before the first is used,
-  // the exponentials have one reference, and the selection's bound comes from all of them.
-  u32x4 raw[kBatches][kLoads];
-  for (int v = v0; v < v1; v += kBatches * kBatch) {
-#pragma unroll
-    for (int i = 0; i < kBatches; ++i)
-      if (v + i * kBatch < v1) load(raw[i], v + i * kBatch);
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kBatches; ++i) {
-      if (v + i * kBatch >= v1) break;
-#pragma unroll
-      for (int e = 0; e < kElems; ++e) most = fmaxf(most, logit(raw[i], e));
-    }
-    const float top = fmaxf(m, most), use = top == -INFINITY ? 0.f : top;
-    sum *= (double)fast_exp2((m - use) * kLog2e);
-    m = top;
-#pragma unroll
-    for (int i = 0; i < kBatches; ++i) {
-      if (v + i * kBatch >= v1) break;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2((logit(raw[i], e) - use) * kLog2e);
-      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
-    }
-    if (v == v0 || __builtin_amdgcn_ballot_w64(most > tau)) select(raw, v, most);
   }
-  // Over the lanes: relative to the largest maximum.
-  const float top = wave_fmaxf(m);
-  if (__builtin_amdgcn_ballot_w64(sum != sum)) {  // NaN or +inf among the logits: once more, with care
+  if (c >= p.chunks) return;
+  // Over the lanes.  Where a logit is NaN or +inf, or so large that the reference's rounding is more than the
+  // exponent's, once more with care, relative to the largest.
+  const bool careful = __builtin_amdgcn_ballot_w64(sum != sum) || !(fabsf(top) <= 4096.f || top == -INFINITY);
+  if (careful) {
     sum = 0;
     for (int t = v0 + lane; t < v1; t += 64) {
       const float x = fmaxf(BF16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(src)[t]) : reinterpret_cast<const float*>(src)[t],
                             -INFINITY);
       sum += x == top ? 1.0 : exp((double)x - (double)top);
     }
-  } else {
-    sum = m == -INFINITY ? 0.0 : sum * exp((double)m - (double)top);
   }
   sum = wave_sum64(sum);
 
-  uint64_t* keys = reinterpret_cast<uint64_t*>(p.ws) + (int64_t)row * p.chunks * (beams + 2);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(p.ws) + (int64_t)row * p.chunks * (beams + kStats);
   if (lane < beams) keys[(int64_t)lane * p.chunks + c] = best.key;  // [place][chunk]
   double* stats = reinterpret_cast<double*>(keys + (int64_t)beams * p.chunks);
   if (lane == 0) {
     stats[c] = (double)top;
     stats[p.chunks + c] = sum;
+    stats[2 * p.chunks + c] = careful ? __builtin_nan("") : (double)ref;  // sum * 2^ref, or (NaN) sum * e^top
   }
 }
 
@@ -240,11 +268,12 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x, beams = p.beams, chunks = p.chunks;
   for (int w = wave; w < p.width; w += (int)(blockDim.x >> 6)) {
-    const uint64_t* keys = reinterpret_cast<const uint64_t*>(p.ws) + ((int64_t)b * p.width + w) * chunks * (beams + 2);
+    const uint64_t* keys = reinterpret_cast<const uint64_t*>(p.ws) + ((int64_t)b * p.width + w) * chunks * (beams + kStats);
     const double* stats = reinterpret_cast<const double*>(keys + (int64_t)beams * chunks);
     const bool mine = lane < chunks;
     const double m = mine ? stats[lane] : -(double)INFINITY;
     double sum = mine ? stats[chunks + lane] : 0.0;
+    const double ref = mine ? stats[2 * chunks + lane] : 0.0;
     const float score = p.scores[(int64_t)b * p.width + w];
     // The chunks' lists are sorted: their first keys, then the second ones, ... while any is better
     // than the last taken.  Four places are on their way at a time.
@@ -259,7 +288,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
         uint64_t least = bcast(best.key, beams - 1);
         uint64_t mask = __builtin_amdgcn_ballot_w64(k[i] > least);
         if (__popcll(mask) > beams) {  // none below the beams-th largest matters
-          const uint32_t bound = nth_bound((uint32_t)(k[i] >> 32), beams);
+          const uint32_t x[1] = {(uint32_t)(k[i] >> 32)};
+          uint32_t unused;
+          const uint32_t bound = nth_bound(x, beams, unused);
           mask = __builtin_amdgcn_ballot_w64(k[i] > least && (uint32_t)(k[i] >> 32) >= bound);
         }
         more = mask != 0;
@@ -272,7 +303,10 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     }
     if (lane < beams) row_keys[w * beams + lane] = best.key;
     const double top = (double)wave_fmaxf((float)m);
-    sum = wave_sum64(m == top ? sum : sum * exp(m - top));
+    // Relative to the row's largest.  The scan's log2(e) is the f32 constant, and so it is here: what that is off by
+    // then counts for the distance to the largest only.
+    const double power = ref != ref ? (m - top) * 1.4426950408889634 : ref - top * (double)kLog2e;
+    sum = wave_sum64(sum == 0.0 || (ref != ref && m == top) ? sum : sum * exp2(power));
     if (lane == 0) {
       row_max[w] = top;
       row_add[w] = (double)score - log(sum);
@@ -336,14 +370,13 @@ int beam_chunks(int batch, int width, int vocab, int* size) {
 
 int64_t beam_ws_bytes(int batch, int width, int vocab, int beams) {
   int size;
-  return (int64_t)batch * width * beam_chunks(batch, width, vocab, &size) * (beams + 2) * 8;
+  return (int64_t)batch * width * beam_chunks(batch, width, vocab, &size) * (beams + kStats) * 8;
 }
 
 hipError_t launch_beam_select(const BeamParams& params, hipStream_t stream) {
   BeamParams p = params;
   p.chunks = beam_chunks(p.batch, p.width, p.vocab, &p.chunk_size);
-  const int64_t waves = (int64_t)p.batch * p.width * p.chunks;
-  const dim3 grid((unsigned)((waves + kScanWaves - 1) / kScanWaves)), block(kScanWaves * 64);
+  const dim3 grid((unsigned)((int64_t)p.batch * p.width * ((p.chunks + kScanWaves - 1) / kScanWaves))), block(kScanWaves * 64);
   if (p.bf16) hipLaunchKernelGGL(beam_scan_kernel<true>, grid, block, 0, stream, p);
   else hipLaunchKernelGGL(beam_scan_kernel<false>, grid, block, 0, stream, p);
   const int join = p.width < kJoinWaves ? p.width : kJoinWaves;
