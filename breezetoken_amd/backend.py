@@ -828,11 +828,14 @@ class HipBackend:
 
     # ------------------------------------------------------------ paged caches
     # Workspaces here are allocated by each call on its stream, from torch's
-    # allocator: calls on two streams, or two captured graphs, share none.
+    # allocator: calls on two streams, or two captured graphs, share none.  Small
+    # calls take as long as this host path (12 to 16 us of which 3 are a launch),
+    # so each tensor's checks are one expression, and outputs are made like an
+    # input where one fits (1.2 us; torch.empty with a type and device 1.7).
     def _run(self, name: str, *args) -> None:
         """Launch on this backend's device, whichever is current."""
         fn, dev = getattr(self._lib, name), self._dev
-        if torch.cuda.current_device() == dev.index:
+        if torch._C._cuda_getDevice() == dev.index:
             rc = fn(*args, _stream(dev))
         else:
             with torch.cuda.device(dev):
@@ -840,37 +843,40 @@ class HipBackend:
         if rc:
             check(name, rc)
 
-    def _on_device(self, **tensors: torch.Tensor | None) -> None:
-        for name, t in tensors.items():
-            if t is not None and t.device != self._dev:
-                raise RuntimeError(f"{name} must live on the backend's device")
-
-    @staticmethod
-    def _check_ints(name: str, t: torch.Tensor, n: int) -> None:
+    def _ints(self, name: str, t: torch.Tensor, n: int) -> int:
+        """Address of a contiguous int32 device tensor of n values."""
         if t.dtype is not torch.int32 or t.ndim != 1 or t.shape[0] != n or not t.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} values")
+        if t.device != self._dev:
+            raise RuntimeError(f"{name} must live on the backend's device")
+        return t.data_ptr()
 
-    @staticmethod
-    def _check_table(table: torch.Tensor) -> None:
+    def _page_table(self, table: torch.Tensor) -> tuple[int, int]:
+        """Rows and entries per row of a page table."""
         if table.dtype is not torch.int32 or table.ndim != 2 or not table.is_contiguous() or table.shape[1] < 1:
             raise RuntimeError("table must be a contiguous int32 (rows, pages) tensor")
+        if table.device != self._dev:
+            raise RuntimeError("table must live on the backend's device")
+        return table.shape
 
     def _paged_kv(self, k: torch.Tensor, v: torch.Tensor, dim: int) -> tuple[int, int, int, int, int, int]:
         """Pages, page size, kv heads and the strides of a page, token and head."""
-        if k.ndim != 4 or v.shape != k.shape:
+        shape, stride = k.shape, k.stride()
+        if len(shape) != 4 or v.shape != shape:
             raise RuntimeError("k/v must be (pages, page_size, Hkv, D) with equal shapes")
-        pages, size, groups, kdim = k.shape
+        pages, size, groups, kdim = shape
         if kdim != dim or groups < 1 or pages < 1:
-            raise RuntimeError(f"a cache {tuple(k.shape)} does not hold heads of {dim}")
+            raise RuntimeError(f"a cache {tuple(shape)} does not hold heads of {dim}")
         if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
             raise RuntimeError("the MI355X path serves a bf16 KV cache only")
+        if k.device != self._dev or v.device != self._dev:
+            raise RuntimeError("k/v must live on the backend's device")
         if size not in PAGE_SIZES:
             raise RuntimeError(f"page size {size} is not served {PAGE_SIZES}")
-        sp, st, sh, sd = k.stride()
-        if sd != 1 or v.stride() != k.stride():
+        if stride[3] != 1 or v.stride() != stride:
             raise RuntimeError("k/v need unit d-stride and identical strides")
         # The stride of a dimension of one is whatever its maker left there.
-        return pages, size, groups, sp if pages > 1 else size * groups * dim, st, sh if groups > 1 else dim
+        return pages, size, groups, stride[0] if pages > 1 else size * groups * dim, stride[1], stride[2] if groups > 1 else dim
 
     def attention_paged(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
                         lens: torch.Tensor, scale: float, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -889,22 +895,23 @@ class HipBackend:
             raise RuntimeError(f"q heads {heads} / kv heads {groups} do not form a GQA group")
         if dim not in SERVED_HEAD_DIMS or heads // groups > MAX_GROUP:
             raise RuntimeError(f"shape H={heads} Hkv={groups} D={dim} is not served")
-        self._check_table(table)
-        if table.shape[0] != batch:
+        rows, per_seq = self._page_table(table)
+        if rows != batch:
             raise RuntimeError("table needs one row per sequence")
-        self._check_ints("lens", lens, batch)
-        self._on_device(q=q, k=k, v=v, table=table, lens=lens)
+        lens_ptr = self._ints("lens", lens, batch)
+        if q.device != self._dev:
+            raise RuntimeError("q must live on the backend's device")
         q_code, out_code = _dtype_code(q.dtype), _dtype_code(out_dtype)
-        out = torch.empty((batch, heads, dim), dtype=out_dtype, device=self._dev)
+        q = q.contiguous()
+        out = torch.empty_like(q, dtype=out_dtype)
         if batch == 0:
             return out
-        q = q.contiguous()
-        per_seq = table.shape[1]
         nbytes = self._lib.bt_paged_workspace_bytes(batch, heads, groups, dim, min(per_seq * size, 0x7FFFFFFF))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev) if nbytes else None
-        self._run("bt_gqa_decode_paged", q.data_ptr(), q_code, heads * dim, k.data_ptr(), v.data_ptr(), sp, st, sh, pages,
-                  size, table.data_ptr(), per_seq, per_seq, lens.data_ptr(), batch, heads, groups, dim, float(scale),
-                  _ptr(ws), nbytes, out.data_ptr(), out_code, heads * dim)
+        ws = lens.new_empty(nbytes >> 2) if nbytes else None
+        row = heads * dim
+        self._run("bt_gqa_decode_paged", q.data_ptr(), q_code, row, k.data_ptr(), v.data_ptr(), sp, st, sh, pages, size,
+                  table.data_ptr(), per_seq, per_seq, lens_ptr, batch, heads, groups, dim, float(scale),
+                  ws.data_ptr() if nbytes else None, nbytes, out.data_ptr(), out_code, row)
         return out
 
     def attn_prep_paged(
@@ -930,19 +937,20 @@ class HipBackend:
             raise RuntimeError(f"head_dim {D} is not served {SERVED_PREP_DIMS}")
         if heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise RuntimeError(f"q heads {heads} / kv heads {kv_heads} do not form a GQA group")
-        nq = heads * D * (2 if gated else 1)
-        if qkv.ndim != 2 or qkv.shape[1] != nq + 2 * kv_heads * D:
-            raise RuntimeError(f"qkv {tuple(qkv.shape)} is not (T, {nq + 2 * kv_heads * D})")
+        width = heads * D * (2 if gated else 1) + 2 * kv_heads * D
+        if qkv.ndim != 2 or qkv.shape[1] != width:
+            raise RuntimeError(f"qkv {tuple(qkv.shape)} is not (T, {width})")
+        if qkv.device != self._dev:
+            raise RuntimeError("qkv must live on the backend's device")
         tokens = qkv.shape[0]
         pages, size, groups, sp, st, sh = self._paged_kv(k, v, D)
         if groups != kv_heads:
             raise RuntimeError(f"the cache holds {groups} kv heads, not {kv_heads}")
-        self._check_table(table)
-        self._check_ints("pos", pos, tokens)
-        if rows is not None:
-            self._check_ints("rows", rows, tokens)
-        elif table.shape[0] < tokens:
+        table_rows, per_seq = self._page_table(table)
+        pos_ptr = self._ints("pos", pos, tokens)
+        if rows is None and table_rows < tokens:
             raise RuntimeError("table needs a row per token where rows is not given")
+        rows_ptr = None if rows is None else self._ints("rows", rows, tokens)
         if (q_norm is None) != (k_norm is None) or (cos is None) != (sin is None):
             raise RuntimeError("q_norm and k_norm, and cos and sin, are given together")
         if q_norm is not None:
@@ -950,48 +958,58 @@ class HipBackend:
             self._check_f32_dev("k_norm", k_norm)
             if q_norm.numel() != D or k_norm.numel() != D:
                 raise ValueError("q_norm/k_norm must hold head_dim values")
-            q_norm, k_norm = q_norm.reshape(-1).contiguous(), k_norm.reshape(-1).contiguous()
+            if not (q_norm.is_contiguous() and k_norm.is_contiguous()):
+                q_norm, k_norm = q_norm.contiguous(), k_norm.contiguous()
         cap = 1
-        if cos is not None:
+        if cos is None:
+            rope_dim = 0
+        else:
             rope_dim = operator.index(rope_dim)
             if rope_dim < 2 or rope_dim % 2 or rope_dim > D:
                 raise ValueError(f"invalid rope_dim {rope_dim} for rows of {D}")
-            for n, t in (("cos", cos), ("sin", sin)):
-                self._check_f32_dev(n, t)
-                if t.ndim != 2 or t.shape[1] != rope_dim or not t.is_contiguous():
-                    raise RuntimeError(f"{n} must be a contiguous (cap, rope_dim) table")
+            self._check_f32_dev("cos", cos)
+            self._check_f32_dev("sin", sin)
+            if cos.ndim != 2 or cos.shape[1] != rope_dim or not cos.is_contiguous() or not sin.is_contiguous():
+                raise RuntimeError("cos and sin must be contiguous (cap, rope_dim) tables")
             if sin.shape != cos.shape or cos.shape[0] < 1:
                 raise RuntimeError("cos and sin tables differ in shape, or are empty")
             cap = cos.shape[0]
-        self._on_device(qkv=qkv, pos=pos, rows=rows, k=k, v=v, table=table)
         code, q_code = _dtype_code(qkv.dtype), _dtype_code(q_dtype)
-        if qkv.stride(1) != 1 or qkv.stride(0) < qkv.shape[1] or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+        step, unit = qkv.stride()
+        if unit != 1 or step < width or step % 8 or qkv.data_ptr() % 16:
             qkv = qkv.contiguous()
-        q = torch.empty((tokens, heads, D), dtype=q_dtype, device=self._dev)
+            step = width
+        q = qkv.new_empty((tokens, heads, D), dtype=q_dtype)
         if tokens:
-            self._run("bt_attn_prep_paged", qkv.data_ptr(), code, qkv.stride(0), tokens, heads, kv_heads, D, int(gated),
-                      _ptr(q_norm), _ptr(k_norm), float(eps), _ptr(cos), _ptr(sin), rope_dim if cos is not None else 0,
-                      cap, int(interleaved), pos.data_ptr(), _ptr(rows), q.data_ptr(), q_code, k.data_ptr(),
-                      v.data_ptr(), sp, st, sh, pages, size, table.data_ptr(), table.shape[1], table.shape[0],
-                      table.shape[1])
-        return q, qkv[:, :nq].view(tokens, heads, 2 * D)[..., D:] if gated else None
+            self._run("bt_attn_prep_paged", qkv.data_ptr(), code, step, tokens, heads, kv_heads, D, int(gated),
+                      _ptr(q_norm), _ptr(k_norm), float(eps), _ptr(cos), _ptr(sin), rope_dim, cap, int(interleaved),
+                      pos_ptr, rows_ptr, q.data_ptr(), q_code, k.data_ptr(), v.data_ptr(), sp, st, sh, pages, size,
+                      table.data_ptr(), per_seq, table_rows, per_seq)
+        if not gated:
+            return q, None
+        return q, qkv.as_strided((tokens, heads, D), (step, 2 * D, 1), qkv.storage_offset() + D)
 
     def _page_args(self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor | None):
+        """The page operators' common arguments: those of the pages, of the table before, and of ``keep``."""
         if pages.dtype is not torch.bfloat16 or pages.ndim != 4 or pages.shape[0] < 1 or pages.shape[1] < 1:
             raise RuntimeError("pages must be a bf16 (planes, pages, page_size, Hkv * D) tensor")
+        if pages.device != self._dev:
+            raise RuntimeError("pages must live on the backend's device")
         planes, num, size, width = pages.shape
         if size not in PAGE_SIZES:
             raise RuntimeError(f"page size {size} is not served {PAGE_SIZES}")
-        if width < 8 or width % 8 or pages.stride(3) != 1 or pages.stride(2) != width:
+        plane_stride, page_stride, token_stride, unit = pages.stride()
+        if width < 8 or width % 8 or unit != 1 or token_stride != width:
             raise RuntimeError("each page must be contiguous, Hkv * D a multiple of 8")
-        page_stride = pages.stride(1) if num > 1 else size * width
-        plane_stride = pages.stride(0) if planes > 1 else num * page_stride
-        self._check_table(table)
-        self._check_ints("lens", lens, table.shape[0])
-        if keep is not None:
-            self._check_ints("keep", keep, keep.numel())
-        self._on_device(pages=pages, table=table, lens=lens, keep=keep)
-        return pages.data_ptr(), plane_stride, page_stride, planes, num, size, width
+        if num == 1:
+            page_stride = size * width
+        if planes == 1:
+            plane_stride = num * page_stride
+        rows, per_seq = self._page_table(table)
+        lens_ptr = self._ints("lens", lens, rows)
+        kept = (None, 0) if keep is None else (self._ints("keep", keep, keep.numel()), keep.numel())
+        return ((pages.data_ptr(), plane_stride, page_stride, planes, num, size, width),
+                (table.data_ptr(), lens_ptr, rows, per_seq), kept)
 
     def fork_pages(
         self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent: torch.Tensor | None = None,
@@ -1010,27 +1028,27 @@ class HipBackend:
         without the added tokens, status (2,) int32 = pages left free and pages that
         could not be given -- their entries are -1, and the old table still names
         what the new rows would lose, so the step can be taken again."""
-        args = self._page_args(pages, table, lens, keep)
-        rows_in, per_seq = table.shape
-        rows = rows_in
-        if parent is not None:
+        args, before, kept = self._page_args(pages, table, lens, keep)
+        rows_in, per_seq = before[2], before[3]
+        if parent is None:
+            rows, parent_ptr = rows_in, None
+        else:
             rows = parent.numel()
-            self._check_ints("parent", parent, rows)
-        if not isinstance(add, torch.Tensor):
+            parent_ptr = self._ints("parent", parent, rows)
+        if isinstance(add, torch.Tensor):
+            add_ptr = self._ints("add", add, rows)
+        else:
             n = operator.index(add)
             if not 0 <= n <= 0x7FFFFFFF:
                 raise ValueError(f"add must not be negative or over 2^31 - 1, got {n}")
             add = torch.full((rows,), n, dtype=torch.int32, device=self._dev) if n else None
-        else:
-            self._check_ints("add", add, rows)
-        self._on_device(parent=parent, add=add)
-        new = torch.empty((rows, per_seq), dtype=torch.int32, device=self._dev)
-        new_lens = torch.empty(rows, dtype=torch.int32, device=self._dev)
-        status = torch.empty(2, dtype=torch.int32, device=self._dev)
-        nbytes = self._lib.bt_pages_workspace_bytes(args[4], max(rows, rows_in))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
-        self._run("bt_fork_pages", *args, table.data_ptr(), lens.data_ptr(), rows_in, per_seq, _ptr(parent), _ptr(add), rows,
-                  _ptr(keep), 0 if keep is None else keep.numel(), new.data_ptr(), new_lens.data_ptr(),
+            add_ptr = _ptr(add)
+        new = table.new_empty((rows, per_seq))
+        new_lens = lens.new_empty(rows)
+        status = lens.new_empty(2)
+        nbytes = self._lib.bt_pages_workspace_bytes(args[4], rows)
+        ws = lens.new_empty(nbytes >> 2)
+        self._run("bt_fork_pages", *args, *before, parent_ptr, add_ptr, rows, *kept, new.data_ptr(), new_lens.data_ptr(),
                   status.data_ptr(), ws.data_ptr(), nbytes)
         return new, new_lens, status
 
@@ -1041,16 +1059,14 @@ class HipBackend:
         ``keep`` names (arguments as ``fork_pages``).  Returns (table, where, live): the
         new table, the new place of every page ((pages,) int32, -1: free; for other
         tables and ``keep``), and the number of live pages ((1,) int32)."""
-        args = self._page_args(pages, table, lens, keep)
-        rows, per_seq = table.shape
+        args, before, kept = self._page_args(pages, table, lens, keep)
         new = torch.empty_like(table)
-        where = torch.empty(args[4], dtype=torch.int32, device=self._dev)
-        live = torch.empty(1, dtype=torch.int32, device=self._dev)
-        nbytes = self._lib.bt_pages_workspace_bytes(args[4], rows)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
-        self._run("bt_compact_pages", *args, table.data_ptr(), lens.data_ptr(), rows, per_seq, _ptr(keep),
-                  0 if keep is None else keep.numel(), new.data_ptr(), where.data_ptr(), live.data_ptr(), ws.data_ptr(),
-                  nbytes)
+        where = lens.new_empty(args[4])
+        live = lens.new_empty(1)
+        nbytes = self._lib.bt_pages_workspace_bytes(args[4], before[2])
+        ws = lens.new_empty(nbytes >> 2)
+        self._run("bt_compact_pages", *args, *before, *kept, new.data_ptr(), where.data_ptr(), live.data_ptr(),
+                  ws.data_ptr(), nbytes)
         return new, where, live
 
     def beam_select(
@@ -1064,29 +1080,33 @@ class HipBackend:
         beams) int32).  Compared in 64 bits; ties go to the lower beam, then to the
         lower token.  A barred token has the logit -inf (NaN counts as that); a beam
         that has ended keeps its score with one logit of 0 and -inf elsewhere."""
-        if logits.ndim != 3 or scores.shape != logits.shape[:2]:
+        shape = logits.shape
+        if len(shape) != 3 or scores.shape != shape[:2]:
             raise RuntimeError("beam_select expects logits (B, W, V) and scores (B, W)")
-        batch, width, vocab = logits.shape
+        batch, width, vocab = shape
         beams = width if beams is None else operator.index(beams)
         if vocab < 1 or width < 1 or not 1 <= beams <= width * vocab:
             raise ValueError(f"{beams} beams cannot be taken from {width} x {vocab} candidates")
         if width > MAX_BEAMS or beams > MAX_BEAMS:
             raise RuntimeError(f"more than {MAX_BEAMS} beams are not served")
         code = _dtype_code(logits.dtype)
+        if logits.device != self._dev:
+            raise RuntimeError("logits must live on the backend's device")
         self._check_f32_dev("scores", scores)
-        self._on_device(logits=logits)
-        if logits.stride(2) != 1:
+        stride = logits.stride()
+        if stride[2] != 1:
             logits = logits.contiguous()
+            stride = logits.stride()
         scores = scores.contiguous()
-        best = torch.empty((batch, beams), dtype=torch.float32, device=self._dev)
-        parent = torch.empty((batch, beams), dtype=torch.int32, device=self._dev)
-        token = torch.empty((batch, beams), dtype=torch.int32, device=self._dev)
+        best = scores.new_empty((batch, beams))
+        parent = torch.empty_like(best, dtype=torch.int32)
+        token = torch.empty_like(parent)
         if batch == 0:
             return best, parent, token
         nbytes = self._lib.bt_beam_workspace_bytes(batch, width, vocab, beams)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
-        self._run("bt_beam_select", logits.data_ptr(), code, logits.stride(0), logits.stride(1), scores.data_ptr(), batch,
-                  width, vocab, beams, best.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), nbytes)
+        ws = token.new_empty(nbytes >> 2)
+        self._run("bt_beam_select", logits.data_ptr(), code, stride[0], stride[1], scores.data_ptr(), batch, width, vocab,
+                  beams, best.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), nbytes)
         return best, parent, token
 
     def close(self) -> None:

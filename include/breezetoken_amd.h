@@ -424,8 +424,8 @@ int bt_attn_prep_paged(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, i
                        const int32_t* table, int64_t table_stride, int32_t table_rows, int32_t pages_per_seq,
                        void* stream);
 
-/* Bytes of workspace bt_fork_pages and bt_compact_pages need, `rows` the larger of
- * the rows they read and write. */
+/* Bytes of workspace bt_fork_pages and bt_compact_pages need for `rows` rows of
+ * their result. */
 int64_t bt_pages_workspace_bytes(int32_t num_pages, int32_t rows);
 
 /* Sequences that continue others in a paged cache, with room for their next
