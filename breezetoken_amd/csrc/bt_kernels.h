@@ -420,8 +420,8 @@ struct PagedDecodeParams {
   const int32_t* lens;  // (batch,) valid keys
   int32_t batch, heads, kv_heads, group;
   float scale_log2;
-  int32_t runs;  // work-groups per kv head, paged_runs()
-  // Parts of sequences that lie in several runs (runs > 1): rows of runs + batch
+  int32_t runs;  // work-groups per kv head, paged_runs(); 0: one for each sequence
+  // Parts of sequences that lie in several runs: rows of runs + batch
   // slots per head, and each sequence's first slot and their number.
   float* lse;
   float* part;

@@ -72,7 +72,7 @@ struct PagedWorkspace {
 PagedWorkspace paged_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens) {
   PagedWorkspace w{};
   w.runs = bt::paged_runs(batch, kv_heads, head_dim, max_tokens, device_cus());
-  if (w.runs == 1) return w;
+  if (w.runs == 0) return w;
   const int64_t slots = (int64_t)heads * (w.runs + batch);
   w.part = align256(slots * 4);
   w.base = w.part + align256(slots * head_dim * 4);

@@ -14,7 +14,8 @@
 // a sequence writes its result; the parts of a sequence cut by a run's end go to
 // the workspace as (lse, normalised partial) and the combine joins them.  The
 // part of work-group w in sequence b has slot w + b: runs and sequences both
-// advance in order, so slots are unique and a sequence's are consecutive.
+// advance in order, so slots are unique and a sequence's are consecutive.  Where the
+// tables are short (paged_runs) a work-group takes a sequence, and nothing is joined.
 //
 // Within a work-group the waves take a run's tiles in turn, each with an online
 // softmax of its own, merged through LDS where a sequence ends.  A wave's next
@@ -61,11 +62,11 @@ struct Window {
   int first;  // sequence of lane 0
   int start;  // tiles before it
   int len, ends;
-  __device__ __forceinline__ void load(const PagedDecodeParams& p, int f, int s, int cap) {
+  __device__ __forceinline__ void load(const PagedDecodeParams& p, int f, int s, int cap, int count = 64) {
     first = f;
     start = s;
     const int b = f + (int)(threadIdx.x & 63);
-    len = b < p.batch ? p.lens[b] : 0;
+    len = b < p.batch && (int)(threadIdx.x & 63) < count ? p.lens[b] : 0;
     len = len < 0 ? 0 : (len > cap ? cap : len);
     int x = (len + 15) >> 4;
 #pragma unroll
@@ -109,11 +110,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   const int cap = p.pg.pages_per_seq << p.pg.page_shift;
 
   // ---- the batch's tiles and this work-group's run ---------------------------
-  const int windows = (p.batch + 63) >> 6;  // at most 64
+  const bool whole = p.runs == 0;  // work-group w takes sequence w, numbered alone
+  const int windows = whole ? 1 : (p.batch + 63) >> 6;  // at most 64
   Window win;  // of the tile looked at last
   int wends = 0, total;
   if (windows == 1) {
-    win.load(p, 0, 0, cap);
+    win.load(p, whole ? w : 0, 0, cap, whole ? 1 : 64);
     total = bcast(win.ends, 63);
   } else {
     for (int i = wave; i < windows; i += kWaves) {
@@ -139,12 +141,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   int runs = (total + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
   runs = runs < 1 ? 1 : (runs < p.runs ? runs : p.runs);
   const int share = total ? (total + runs - 1) / runs : 1;
-  const int t0 = w * share < total ? w * share : total;
-  const int t1 = t0 + share < total ? t0 + share : total;
+  const int t0 = whole ? 0 : (w * share < total ? w * share : total);
+  const int t1 = whole || t0 + share > total ? total : t0 + share;
 
   // The last work-group of the first head, often an idle one, says where each
   // sequence's parts are: their number (1: the result is written) and first slot.
-  if (w == p.runs - 1 && kvh == 0 && p.runs > 1) {
+  if (w == p.runs - 1 && kvh == 0) {
     for (int i = wave; i < windows; i += kWaves) {
       if (windows > 1) win.load(p, 64 * i, i ? bcast(wends, i - 1) : 0, cap);
       const int b = 64 * i + lane, n = (win.len + 15) >> 4;
@@ -166,11 +168,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
       *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row) = a;
     }
   };
-  if (p.runs == 1) {  // no combine follows: sequences without keys are zeroed here
-    for (int i = 0; i < p.batch * G * (D / 4); i += kThreads) {
-      const int item = i + threadIdx.x, b = item / (G * (D / 4)), r = item % (G * (D / 4));
-      if (b < p.batch && p.lens[b] <= 0) store_out(b, r / (D / 4), r % (D / 4) * 4, float4{0.f, 0.f, 0.f, 0.f});
-    }
+  if (whole && total == 0) {  // no combine follows
+    for (int item = threadIdx.x; item < G * (D / 4); item += kThreads)
+      store_out(w, item / (D / 4), item % (D / 4) * 4, float4{0.f, 0.f, 0.f, 0.f});
   }
   if (t0 >= t1) return;
 
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
 
 template <int GMAX, int D>
 hipError_t launch_dim(const PagedDecodeParams& p, hipStream_t stream) {
-  const dim3 grid(p.runs * p.kv_heads), block(kWaves * 64);
+  const dim3 grid((p.runs ? p.runs : p.batch) * p.kv_heads), block(kWaves * 64);
   if (p.q_bf16) {
     if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, false>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, true>), grid, block, 0, stream, p);
@@ -487,7 +487,13 @@ hipError_t launch_dim(const PagedDecodeParams& p, hipStream_t stream) {
 
 int paged_runs(int batch, int kv_heads, int head_dim, int64_t max_tokens, int num_cus) {
   const int64_t most = (int64_t)batch * ((max_tokens + 15) / 16);  // tiles of the largest call
-  if (batch * max_tokens * head_dim <= 32768) return 1;
+  // Short tables: a work-group per sequence, which writes its result, and no combine.
+  // us a graph node (issued one by one), whole sequences / runs, D = 256, Hkv = 2: one
+  // sequence of 128 tokens 7.3 (9.4) / 8.6 (13.5), 256 8.8 (9.6) / 8.6 (13.6), 512 11.9
+  // (11.7) / 8.7 (13.4); 128 sequences of 256 13.7 / 19.1; D = 128, Hkv = 8: one of 512
+  // 9.1 (9.6) / 8.5 (13.7), 1,024 12.8 (12.7) / 8.9 (13.7), 128 of 512 58 / 62; D = 64,
+  // Hkv = 4: one of 512 7.1 (9.6) / 7.3 (13.7), 1,024 10.2 (10.1) / 7.4 (13.7).
+  if (max_tokens <= 512 && max_tokens * head_dim <= 65536) return 0;
   const int per_cu = head_dim == 256 ? 1 : 2;
   int64_t runs = (int64_t)num_cus * per_cu / kv_heads;
   const int64_t enough = (most + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
@@ -504,7 +510,7 @@ hipError_t launch_decode_paged(const PagedDecodeParams& p, int head_dim, hipStre
     case 256: e = small ? launch_dim<4, 256>(p, stream) : launch_dim<8, 256>(p, stream); break;
     default: return hipErrorInvalidValue;
   }
-  if (e != hipSuccess || p.runs == 1) return e;
+  if (e != hipSuccess || p.runs == 0) return e;
   CombineParams c{};
   c.lse = p.lse;
   c.part = p.part;
