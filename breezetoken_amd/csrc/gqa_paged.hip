@@ -47,12 +47,13 @@ __device__ __forceinline__ float term_sum(float v) {
   return v;
 }
 
-// The 16-byte slot of a tile's row that holds chunk c is c ^ slot_of(row): linear in
-// the row's bits, and such that the operand reads of K (16 rows, one chunk) and the
-// transposed reads of V (8 rows, a pair of chunks) fall on distinct banks.
+// The 16-byte slot of a tile's row that holds chunk c is c ^ slot_of(row): linear in the
+// row's bits, and without bank conflicts (measured) both for the operand reads of K, whose
+// 16 bytes a lane the LDS serves in groups of lanes 0-3, 12-15, 20-23, 24-27 (and so on),
+// and for the transposed reads of V (8 rows, a pair of chunks).
 template <int D>
 __device__ __forceinline__ constexpr int slot_of(int r) {
-  return D == 64 ? (r >> 1 & 3) << 1 | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
+  return D == 64 ? r & 6 : (r & 7) * 2;
 }
 
 __device__ __forceinline__ int bcast(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
@@ -158,7 +159,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
     }
   }
 
-  const int64_t head_off = (int64_t)kvh * p.pg.stride_head;
   auto store_out = [&](int b, int h, int d, const float4& a) {
     const int64_t row = (int64_t)b * p.out_stride_seq + (int64_t)(head0 + h) * D + d;
     if (p.out_bf16) {
@@ -222,27 +222,35 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   struct Tile {
     int id, rows, token;
   };
+  int seq_tile = 0, seq_end_tile = 0, seq_len = 0;  // of the sequence looked at last: tiles [seq_tile, seq_end_tile)
+  const int32_t* seq_table = p.pg.table;
   auto look_up = [&](int t) -> Tile {
     Tile x{-1, 0, 0};
     if (t < t1) {
-      seek(t);
-      const int i = win.find(t);
-      const int at = (t - win.begin(i)) * 16, b = win.first + i;
-      const int left = bcast(win.len, i) - at;
+      if (t >= seq_end_tile) {
+        seek(t);
+        const int i = win.find(t);
+        seq_tile = win.begin(i);
+        seq_end_tile = bcast(win.ends, i);
+        seq_len = bcast(win.len, i);
+        seq_table = p.pg.table + (int64_t)(win.first + i) * p.pg.table_stride;
+      }
+      const int at = (t - seq_tile) * 16, left = seq_len - at;
       x.rows = left < 16 ? left : 16;
       x.token = at & ((1 << p.pg.page_shift) - 1);
-      x.id = p.pg.table[(int64_t)b * p.pg.table_stride + (at >> p.pg.page_shift)];
+      x.id = uniform_load(seq_table, at >> p.pg.page_shift);
     }
     return x;
   };
   // Points the tile's buffers at its page; returns the rows with keys.
+  const uint16_t* k_head = p.k + (int64_t)kvh * p.pg.stride_head;
+  const uint16_t* v_head = p.v + (int64_t)kvh * p.pg.stride_head;
   auto open = [&](const Tile& x) -> int {
-    const int id = __builtin_amdgcn_readfirstlane(x.id);
-    const bool ok = id >= 0 && id < p.pg.num_pages;
+    const bool ok = (uint32_t)x.id < (uint32_t)p.pg.num_pages;
     const int rows = ok ? x.rows : 0;
-    const int64_t off = ok ? (int64_t)id * p.pg.stride_page + (int64_t)x.token * p.pg.stride_tok + head_off : 0;
-    krs = make_rsrc(p.k + off, (uint32_t)rows * row_bytes);
-    vrs = make_rsrc(p.v + off, (uint32_t)rows * row_bytes);
+    const int64_t off = (int64_t)(ok ? x.id : 0) * p.pg.stride_page + (uint32_t)x.token * (row_bytes / 2);
+    krs = make_rsrc(k_head + off, (uint32_t)rows * row_bytes);
+    vrs = make_rsrc(v_head + off, (uint32_t)rows * row_bytes);
     return rows;
   };
 
@@ -289,12 +297,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   seek(t0);
   load_q(win.first + win.find(t0));
   Tile cur = look_up(t), next = look_up(t + kWaves);
-  int rows = 0;
-  if (t < t1) {
-    rows = open(cur);
-    issue_k();
-    issue_v();
-  }
+  int rows = open(cur);
+  issue_k();
+  issue_v();
 
   const int i16 = lane & 15;
   const int row1 = 4 * kg + (i16 >> 2);  // V^T read: token row of this lane
@@ -318,17 +323,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
     for (int i = 0; i < kDTiles; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
     for (; t < s1; t += kWaves) {
-      const bool more = t + kWaves < t1;
+      // The next tile's requests go out whether there is one or not (none: no rows, nothing is
+      // read), so no branch parts the loads from their waits, which then are for K alone, or the
+      // score MFMAs from the first use of their result: behind a branch hipcc 7.2 puts too few
+      // wait states on the path that takes it, and scores were read before they were there.
       // S^T = K . Q^T, K through the wave's tile into the operand layout.
       floatx4 sacc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
         *reinterpret_cast<BT_LDS u32x4*>((BT_LDS unsigned char*)tile_lds + j * 1024 + lane * 16) = kr[j];
-      int next_rows = 0;
-      if (more) {
-        next_rows = open(next);
-        issue_k();
-      }
+      const int next_rows = open(next);
+      next = look_up(t + 2 * kWaves);
+      issue_k();
       u32x4 kop[kSteps];
       asm volatile("" : "+v"(k_at), "+v"(v_at));
 #pragma unroll
@@ -343,10 +349,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
         *reinterpret_cast<BT_LDS u32x4*>((BT_LDS unsigned char*)tile_lds + j * 1024 + lane * 16) = vr[j];
-      if (more) {
-        issue_v();
-        next = look_up(t + 2 * kWaves);
-      }
+      issue_v();
       // Terms summed, rows without a key masked, online softmax.
       float x[4];
 #pragma unroll
@@ -390,6 +393,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
       rows = next_rows;
     }
 
+    // The last MFMAs' results, wherever the loop was left.
+    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt) asm volatile("" : "+v"(oacc[dt]));
     if (s1 < t1) {  // the next sequence's queries: behind its first tile, which is on its way too
       seek(s1);
       load_q(win.first + win.find(s1));
