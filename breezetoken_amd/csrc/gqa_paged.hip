@@ -58,6 +58,17 @@ __device__ __forceinline__ constexpr int slot_of(int r) {
 
 __device__ __forceinline__ int bcast(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// Inclusive sum over the lanes below, in lane moves (__shfl_up goes through the LDS six times).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
 // 64 sequences' lengths and the batch-wide number of their last tile + 1.
 struct Window {
   int first;  // sequence of lane 0
@@ -66,21 +77,16 @@ struct Window {
   __device__ __forceinline__ void load(const PagedDecodeParams& p, int f, int s, int cap, int count = 64) {
     first = f;
     start = s;
-    const int b = f + (int)(threadIdx.x & 63);
-    len = b < p.batch && (int)(threadIdx.x & 63) < count ? p.lens[b] : 0;
+    const int lane = threadIdx.x & 63;
+    len = f + lane < p.batch && lane < count ? p.lens[f + lane] : 0;
     len = len < 0 ? 0 : (len > cap ? cap : len);
-    int x = (len + 15) >> 4;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o);
-      if ((int)(threadIdx.x & 63) >= o) x += y;
-    }
-    ends = s + x;
+    ends = s + wave_scan((len + 15) >> 4);
   }
   // The lane whose sequence holds tile t (64: a later window).
   __device__ __forceinline__ int find(int t) const { return __popcll(__builtin_amdgcn_ballot_w64(ends <= t)); }
   __device__ __forceinline__ int begin(int lane) const { return lane ? bcast(ends, lane - 1) : start; }
 };
+constexpr int kKeptWindows = 8;  // in LDS; two work-groups of D = 128 still fit a CU
 
 template <int GMAX, int D, bool QBF16, bool F32OUT>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kernel(PagedDecodeParams p) {
@@ -103,6 +109,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   __shared__ __attribute__((aligned(16))) u32x4 qlds[(kSecond ? 2 : 1) * kSteps * 64];
   __shared__ float mstat[2 * kWaves * GMAX];
   __shared__ int wsum[64];
+  __shared__ int2 kept[kKeptWindows * 64];  // len and ends, from the window's own start
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -122,22 +129,30 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
     for (int i = wave; i < windows; i += kWaves) {
       win.load(p, 64 * i, 0, cap);
       if (lane == 63) wsum[i] = win.ends;
+      if (i < kKeptWindows) kept[64 * i + lane] = int2{win.len, win.ends};
     }
     __syncthreads();
-    wends = lane < windows ? wsum[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(wends, o);
-      if (lane >= o) wends += y;
-    }
+    wends = wave_scan(lane < windows ? wsum[lane] : 0);
     total = bcast(wends, 63);
     win.first = -1;
   }
+  auto window = [&](int i) {
+    const int start = i ? bcast(wends, i - 1) : 0;
+    if (i < kKeptWindows) {
+      const int2 x = kept[64 * i + lane];
+      win.first = 64 * i;
+      win.start = start;
+      win.len = x.x;
+      win.ends = start + x.y;
+    } else {
+      win.load(p, 64 * i, start, cap);
+    }
+  };
   // To the window that holds tile t < total.
   auto seek = [&](int t) {
     if (windows == 1) return;
     const int i = __popcll(__builtin_amdgcn_ballot_w64(wends <= t));
-    if (win.first != 64 * i) win.load(p, 64 * i, i ? bcast(wends, i - 1) : 0, cap);
+    if (win.first != 64 * i) window(i);
   };
   int runs = (total + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
   runs = runs < 1 ? 1 : (runs < p.runs ? runs : p.runs);
@@ -149,7 +164,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   // sequence's parts are: their number (1: the result is written) and first slot.
   if (w == p.runs - 1 && kvh == 0) {
     for (int i = wave; i < windows; i += kWaves) {
-      if (windows > 1) win.load(p, 64 * i, i ? bcast(wends, i - 1) : 0, cap);
+      if (windows > 1) window(i);
       const int b = 64 * i + lane, n = (win.len + 15) >> 4;
       if (b < p.batch) {
         const int w0 = (win.ends - n) / share;
