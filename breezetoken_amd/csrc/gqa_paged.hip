@@ -86,10 +86,12 @@ struct Window {
   __device__ __forceinline__ int find(int t) const { return __popcll(__builtin_amdgcn_ballot_w64(ends <= t)); }
   __device__ __forceinline__ int begin(int lane) const { return lane ? bcast(ends, lane - 1) : start; }
 };
-constexpr int kKeptWindows = 8;  // in LDS; two work-groups of D = 128 still fit a CU
+constexpr int kKeptWindows = 8;  // in LDS: 512 sequences; further windows load their lengths again
 
-template <int GMAX, int D, bool QBF16, bool F32OUT>
-__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kernel(PagedDecodeParams p) {
+// WHOLE: work-group w takes sequence w, numbered alone; two of them fit a CU below D =
+// 256 (128 registers).  Runs have a CU each (paged_runs) and take 130 to 195.
+template <int GMAX, int D, bool QBF16, bool F32OUT, bool WHOLE>
+__global__ __launch_bounds__(kWaves * 64, WHOLE && D < 256 ? 4 : 2) void gqa_paged_kernel(PagedDecodeParams p) {
   constexpr int kThreads = kWaves * 64;
   constexpr int kSteps = D / 32;
   constexpr int kDTiles = D / 16;
@@ -118,12 +120,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   const int cap = p.pg.pages_per_seq << p.pg.page_shift;
 
   // ---- the batch's tiles and this work-group's run ---------------------------
-  const bool whole = p.runs == 0;  // work-group w takes sequence w, numbered alone
-  const int windows = whole ? 1 : (p.batch + 63) >> 6;  // at most 64
+  const int windows = WHOLE ? 1 : (p.batch + 63) >> 6;  // at most 64
   Window win;  // of the tile looked at last
   int wends = 0, total;
   if (windows == 1) {
-    win.load(p, whole ? w : 0, 0, cap, whole ? 1 : 64);
+    win.load(p, WHOLE ? w : 0, 0, cap, WHOLE ? 1 : 64);
     total = bcast(win.ends, 63);
   } else {
     for (int i = wave; i < windows; i += kWaves) {
@@ -157,12 +158,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   int runs = (total + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
   runs = runs < 1 ? 1 : (runs < p.runs ? runs : p.runs);
   const int share = total ? (total + runs - 1) / runs : 1;
-  const int t0 = whole ? 0 : (w * share < total ? w * share : total);
-  const int t1 = whole || t0 + share > total ? total : t0 + share;
+  const int t0 = WHOLE ? 0 : (w * share < total ? w * share : total);
+  const int t1 = WHOLE || t0 + share > total ? total : t0 + share;
 
   // The last work-group of the first head, often an idle one, says where each
   // sequence's parts are: their number (1: the result is written) and first slot.
-  if (w == p.runs - 1 && kvh == 0) {
+  if (!WHOLE && w == p.runs - 1 && kvh == 0) {
     for (int i = wave; i < windows; i += kWaves) {
       if (windows > 1) window(i);
       const int b = 64 * i + lane, n = (win.len + 15) >> 4;
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
       *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row) = a;
     }
   };
-  if (whole && total == 0) {  // no combine follows
+  if (WHOLE && total == 0) {  // no combine follows
     for (int item = threadIdx.x; item < G * (D / 4); item += kThreads)
       store_out(w, item / (D / 4), item % (D / 4) * 4, float4{0.f, 0.f, 0.f, 0.f});
   }
@@ -333,6 +334,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
     build_q();
     // Also: every thread is done with the merge of the part before.
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // The next sequence's queries, ahead of further tiles: loads complete in order, and asked for at
+    // this one's end they would be there only when its first tile is, with nothing else on its way.
+    if (!WHOLE && s1 < t1) {
+      seek(s1);
+      load_q(win.first + win.find(s1));
+    }
     floatx4 oacc[kDTiles];
 #pragma unroll
     for (int i = 0; i < kDTiles; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -412,11 +419,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
     asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
 #pragma unroll
     for (int dt = 0; dt < kDTiles; ++dt) asm volatile("" : "+v"(oacc[dt]));
-    if (s1 < t1) {  // the next sequence's queries: behind its first tile, which is on its way too
-      seek(s1);
-      load_q(win.first + win.find(s1));
-    }
-
     // ---- the waves' parts, merged ------------------------------------------------
     l_run = halves_sum(rows16_sum(l_run));
 #pragma unroll
@@ -492,17 +494,22 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void gqa_paged_kerne
   }
 }
 
-template <int GMAX, int D>
-hipError_t launch_dim(const PagedDecodeParams& p, hipStream_t stream) {
-  const dim3 grid((p.runs ? p.runs : p.batch) * p.kv_heads), block(kWaves * 64);
+template <int GMAX, int D, bool WHOLE>
+hipError_t launch_mode(const PagedDecodeParams& p, hipStream_t stream) {
+  const dim3 grid((WHOLE ? p.batch : p.runs) * p.kv_heads), block(kWaves * 64);
   if (p.q_bf16) {
-    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, false>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, true>), grid, block, 0, stream, p);
+    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, false, WHOLE>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, true, WHOLE>), grid, block, 0, stream, p);
   } else {
-    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, false>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, true>), grid, block, 0, stream, p);
+    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, false, WHOLE>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, true, WHOLE>), grid, block, 0, stream, p);
   }
   return hipGetLastError();
+}
+
+template <int GMAX, int D>
+hipError_t launch_dim(const PagedDecodeParams& p, hipStream_t stream) {
+  return p.runs ? launch_mode<GMAX, D, false>(p, stream) : launch_mode<GMAX, D, true>(p, stream);
 }
 
 }  // namespace
@@ -516,8 +523,11 @@ int paged_runs(int batch, int kv_heads, int head_dim, int64_t max_tokens, int nu
   // 9.1 (9.6) / 8.5 (13.7), 1,024 12.8 (12.7) / 8.9 (13.7), 128 of 512 58 / 62; D = 64,
   // Hkv = 4: one of 512 7.1 (9.6) / 7.3 (13.7), 1,024 10.2 (10.1) / 7.4 (13.7).
   if (max_tokens <= 512 && max_tokens * head_dim <= 65536) return 0;
-  const int per_cu = head_dim == 256 ? 1 : 2;
-  int64_t runs = (int64_t)num_cus * per_cu / kv_heads;
+  // One work-group a CU: two (D = 128, 64) keep more requests on their way, and the HBM
+  // serves them less well.  us, one / two: H = 32, Hkv = 8, D = 128, 32 x 8,000 tokens
+  // 166 / 172, 24 x 3,000 53 / 55, one of 131,072 89 / 91; H = 16, Hkv = 2 26 / 34; D =
+  // 64, Hkv = 4, 128 x 2,045 45.5 / 46.8.  (D = 256: two rounds 91, one 84.)
+  int64_t runs = num_cus / kv_heads;
   const int64_t enough = (most + kPagedTilesPerRun - 1) / kPagedTilesPerRun;
   if (runs > enough) runs = enough;
   return runs < 1 ? 1 : (int)runs;

@@ -209,6 +209,165 @@ def test_captured_with_growing_lengths(hip_backend):
         _check(hip_backend, q.cpu(), k.cpu(), v.cpu(), table.cpu(), lens.cpu(), got=out)
 
 
+WIDE = 1024  # tokens a table row has room for: the work is split into runs, at most a work-group each
+
+
+def _wide(lens, H, G, D, page, **kw):
+    return _case(lens, H, G, D, page, per_row=WIDE // page, **kw)
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 256), (15, 5, 64), (7, 1, 128), (16, 4, 128), (4, 1, 256)])
+@pytest.mark.parametrize("q_dtype,out_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                               (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+def test_runs_shapes_and_types(hip_backend, H, G, D, q_dtype, out_dtype):
+    _check(hip_backend, *_wide([1, 37, 1024, 16, 130, 513], H, G, D, 32, q_dtype=q_dtype), out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("lens", [[0], [0, 0, 0], [0, 5, 0, 700, 0], [3, 0], [0, 1], [1024], [1023, 1, 1024],
+                                  [16] * 70, [0] * 65 + [1] + [0] * 64, [17, 0] * 100])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_runs_with_rows_without_tokens(hip_backend, lens, D):
+    q, k, v, table, n = _wide(lens, 8, 2, D, 16)
+    scale = D**-0.5
+    got = hip_backend.attention_paged(q.cuda(), k.cuda(), v.cuda(), table.cuda(), n.cuda(), scale)
+    _check(hip_backend, q, k, v, table, n, got=got)
+    assert not got.cpu()[[i for i, x in enumerate(lens) if x == 0]].any()
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 512, 513, 700, 4096])
+def test_runs_over_many_sequences(hip_backend, batch):
+    """Windows of 64 lengths, the first eight of them kept."""
+    g = torch.Generator().manual_seed(batch)
+    lens = [int(x) for x in torch.exp(torch.rand(batch, generator=g) * 4.0) - 1.0]
+    lens[batch // 2] = 900
+    _check(hip_backend, *_wide(lens, 2, 1, 64, 16, seed=batch))
+
+
+def test_runs_lengths_outside_the_row_are_clamped(hip_backend):
+    q, k, v, table, lens = _wide([1024, 64, 20], 8, 2, 128, 16)
+    lens = torch.tensor([(1 << 31) - 1, -(1 << 31), 20], dtype=torch.int32)
+    clamped = torch.tensor([1024, 0, 20], dtype=torch.int32)
+    ref = orc.attention(q, k, v, table, clamped, 128**-0.5)
+    got = hip_backend.attention_paged(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lens.cuda(), 128**-0.5)
+    _check(hip_backend, q, k, v, table, clamped, ref=ref, got=got)
+
+
+def test_runs_entries_outside_the_cache_hold_no_keys(hip_backend):
+    q, k, v, table, lens = _wide([200, 50, 16, 1000], 8, 2, 128, 16)
+    table[0, 3], table[0, 12] = -1, k.shape[0]
+    table[1, 0] = 1 << 30
+    table[2, 0] = -(1 << 31)  # its only entry: no keys at all
+    got = hip_backend.attention_paged(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lens.cuda(), 128**-0.5)
+    _check(hip_backend, q, k, v, table, lens, got=got)
+    assert not got[2].any()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_runs_do_not_read_slots_without_tokens(hip_backend, D):
+    lens = [5, 33, 48, 250, 1001]
+    q, k, v, table, n = _wide(lens, 8, 2, D, 64, spare=8)
+    ref = orc.attention(q, k, v, table, n, 0.0625)
+    live = torch.zeros(k.shape[:2], dtype=torch.bool)
+    for b, length in enumerate(lens):
+        for t in range(length):
+            live[table[b, t // 64], t % 64] = True
+    bad = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(torch.bfloat16).min])
+    fill = bad[torch.randint(0, 4, k.shape, generator=torch.Generator().manual_seed(9))].to(torch.bfloat16)
+    k2, v2 = torch.where(live[..., None, None], k, fill), torch.where(live[..., None, None], v, fill)
+    got = hip_backend.attention_paged(q.cuda(), k2.cuda(), v2.cuda(), table.cuda(), n.cuda(), 0.0625)
+    tol = orc.attention_tolerance(q, k, v, 0.0625, 1001, ref, False)
+    assert bool(((got.double().cpu() - ref).abs() <= tol).all())
+
+
+def test_runs_nan_query(hip_backend):
+    q, k, v, table, n = _wide([1000, 100], 8, 2, 128, 16)
+    q[0, 3, 5] = float("nan")
+    got = hip_backend.attention_paged(q.cuda(), k.cuda(), v.cuda(), table.cuda(), n.cuda(), 0.1).cpu()
+    assert got[0, 3].isnan().all() and got[1].isfinite().all() and got[0, :3].isfinite().all()
+
+
+def test_runs_large_scores_and_shared_pages(hip_backend):
+    q, k, v, table, n = _wide([900, 17, 640], 8, 2, 128, 32)
+    table[2, :20] = table[0, :20]
+    table[2, 3] = table[2, 0]
+    _check(hip_backend, q * 40, k, v, table, n)
+    q[:] = -30.0
+    k[:] = k.abs()  # every score far below zero
+    _check(hip_backend, q, k, v, table, n)
+
+
+def test_a_sequence_does_not_change_with_its_batch_in_whole_mode(hip_backend):
+    """Short tables: a work-group takes a sequence, so its bits depend on nothing else."""
+    q, k, v, table, n = (t.cuda() for t in _case([300, 7, 512, 0, 64], 8, 2, 128, 16, per_row=32))
+    got = hip_backend.attention_paged(q, k, v, table, n, 0.1)
+    for b in range(5):
+        alone = hip_backend.attention_paged(q[b : b + 1], k, v, table[b : b + 1], n[b : b + 1], 0.1)
+        assert torch.equal(alone[0], got[b])
+
+
+def test_on_another_stream_than_the_current_one(hip_backend):
+    """Tensors made on one stream, used on a second that waits for it, freed while in flight."""
+    side = torch.cuda.Stream()
+    want = None
+    for _ in range(4):
+        args = [t.cuda() for t in _wide([1000, 40, 3], 8, 2, 256, 32)]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = hip_backend.attention_paged(*args, 0.0625)
+        for t in args:
+            t.record_stream(side)
+        del args
+        side.synchronize()
+        want = got if want is None else want
+        assert torch.equal(got, want)
+
+
+def test_two_graphs_replayed_in_turn_and_on_two_streams(hip_backend):
+    a = [t.cuda() for t in _wide([1000, 17], 8, 2, 256, 32, seed=1)]
+    b = [t.cuda() for t in _wide([40, 900, 9], 8, 2, 256, 32, seed=2)]
+    want = hip_backend.attention_paged(*a, 0.0625), hip_backend.attention_paged(*b, 0.0625)
+    graphs, outs = [], []
+    for args in (a, b):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(hip_backend.attention_paged(*args, 0.0625))
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        for i in (0, 1):
+            outs[i].zero_()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_threads_call_at_once(hip_backend):
+    """Four threads, a stream and shapes of their own each; every result is the one alone."""
+    import threading
+
+    cases = [[t.cuda() for t in _wide([700 + 50 * i, 20, 0, 333], 8, 2, 128, 16, seed=i)] for i in range(4)]
+    want = [hip_backend.attention_paged(*c, 0.1) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = hip_backend.attention_paged(*cases[i], 0.1)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_no_sequences(hip_backend):
     q, k, v, table, lens = _case([3], 8, 2, 128, 16)
     got = hip_backend.attention_paged(q[:0].cuda(), k.cuda(), v.cuda(), table[:0].cuda(), lens[:0].cuda(), 0.1)
