@@ -903,6 +903,8 @@ class HipBackend:
             raise RuntimeError("q must live on the backend's device")
         q_code, out_code = _dtype_code(q.dtype), _dtype_code(out_dtype)
         q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
         out = torch.empty_like(q, dtype=out_dtype)
         if batch == 0:
             return out
@@ -977,7 +979,7 @@ class HipBackend:
         code, q_code = _dtype_code(qkv.dtype), _dtype_code(q_dtype)
         step, unit = qkv.stride()
         if unit != 1 or step < width or step % 8 or qkv.data_ptr() % 16:
-            qkv = qkv.contiguous()
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
             step = width
         q = qkv.new_empty((tokens, heads, D), dtype=q_dtype)
         if tokens:

@@ -360,12 +360,13 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
 }  // namespace
 
 // Chunks of a row, at most 64, and their size (whole wave loads): 4,096 waves in all where
-// the rows are long enough, each at least 2,048 logits (a bf16 batch).  us a call, bf16: 128
+// the rows are long enough, each at least 2,048 logits (a bf16 batch), whole work-groups.  us a call, bf16: 128
 // rows of 248,320 26, with 2,048 waves 30; 128 rows of 32,000 13.7 with 1,000 logits a wave,
 // 12.3 with 2,000.
 int beam_chunks(int batch, int width, int vocab, int* size) {
   const int64_t rows = (int64_t)batch * width;
   int64_t want = (4096 + rows - 1) / rows;
+  want = (want + kScanWaves - 1) / kScanWaves * kScanWaves;
   want = want < 64 ? want : 64;
   const int64_t most = ((int64_t)vocab + 2047) / 2048;
   want = want < most ? want : most;

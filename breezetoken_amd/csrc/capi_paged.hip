@@ -106,7 +106,7 @@ int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, co
   if (rc) return rc;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return BT_ENOTSUP;
   if (heads / kv_heads > 8 || batch > bt::kPagedMaxBatch || kv_heads > 65535) return BT_ENOTSUP;
-  if ((int64_t)batch * heads > INT32_MAX / 2) return BT_ENOTSUP;
+  if ((int64_t)batch * heads > INT32_MAX / 512) return BT_ENOTSUP;  // work-items of a launch
   const int64_t max_tokens = (int64_t)pages_per_seq * page_size;
   if (batch * (max_tokens / 16) > INT32_MAX / 2) return BT_ENOTSUP;  // tiles are numbered through the batch
   const PagedWorkspace ws = paged_workspace(batch, heads, kv_heads, head_dim, max_tokens);
@@ -205,7 +205,8 @@ static int page_params(bt::PageOpParams& p, void* pages, int64_t plane_stride, i
   if (rows < 0 || rows_out < 0 || pages_per_seq < 1 || num_keep < 0 || (num_keep && !keep)) return BT_EINVAL;
   if ((rows && (!table || !lens)) || (rows_out && !table_out) || (table_out && table_out == table)) return BT_EINVAL;
   if ((int64_t)pages_per_seq * page_size > INT32_MAX - bt::kMaxPageSize) return BT_ENOTSUP;
-  if ((int64_t)planes * 1024 + (int64_t)rows_out * pages_per_seq + num_keep > INT32_MAX) return BT_ENOTSUP;
+  // Work-items of a launch: 1,024 work-groups of 256 a plane, and one per entry.
+  if ((int64_t)planes * (1024 * 256) + (int64_t)rows_out * pages_per_seq + num_keep > INT32_MAX) return BT_ENOTSUP;
   if ((int64_t)rows * pages_per_seq > INT32_MAX) return BT_ENOTSUP;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bt_pages_workspace_bytes(num_pages, rows_out))
     return BT_ENOSPC;
@@ -271,7 +272,7 @@ int bt_beam_select(const void* logits, int32_t dtype, int64_t stride_batch, int6
   if (!logits || !scores || !scores_out || !parent_out || !token_out) return BT_EINVAL;
   if (batch < 1 || width < 1 || vocab < 1 || beams < 1 || !dtype_known(dtype)) return BT_EINVAL;
   if (stride_batch < 0 || stride_beam < 0 || (int64_t)beams > (int64_t)width * vocab) return BT_EINVAL;
-  if (vocab > (1 << 30) || width > bt::kMaxBeamWidth || beams > bt::kMaxBeams || (int64_t)batch * width > INT32_MAX / 64) return BT_ENOTSUP;
+  if (vocab > (1 << 30) || width > bt::kMaxBeamWidth || beams > bt::kMaxBeams || (int64_t)batch * width > INT32_MAX / 1024) return BT_ENOTSUP;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == BT_DTYPE_BF16 ? 2 : 4)) return BT_EINVAL;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bt_beam_workspace_bytes(batch, width, vocab, beams))
     return BT_ENOSPC;

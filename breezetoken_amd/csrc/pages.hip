@@ -30,7 +30,8 @@ struct Row {
 
 __device__ __forceinline__ int pages_of(const PageOpParams& p, int tokens) { return (tokens + p.page_size - 1) >> p.page_shift; }
 
-// The row that new row r continues, its tokens, and (fork) the entries needed; `over`: entries the table lacks.
+// The row that new row r continues, its tokens, and (fork) the entries needed; `over`: entries the table lacks,
+// at most so many that their sum over the rows fits 31 bits.
 __device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over) {
   const int from = p.parent ? p.parent[r] : r;
   const int cap = p.pages_per_seq * p.page_size;
@@ -43,7 +44,8 @@ __device__ __forceinline__ Row read_row(const PageOpParams& p, int r, int& over)
   const int add = p.add && p.add[r] > 0 ? p.add[r] : 0;
   const int64_t want = ((int64_t)row.n + add + p.page_size - 1) >> p.page_shift;
   row.need = (int)(want < p.pages_per_seq ? want : p.pages_per_seq);
-  over = (int)(want - row.need);
+  const int64_t lacking = want - row.need, most = (1 << 30) / p.rows_out;
+  over = (int)(lacking < most ? lacking : most);
   // Rows without new tokens write nowhere: marked by need = -1 - need.
   if (add == 0) row.need = -1 - row.need;
   return row;
@@ -249,7 +251,8 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
     l.copies[0] = p.rows_out;
     l.copies[1] = free_pages;
     p.status[0] = given < free_pages ? free_pages - given : 0;
-    p.status[1] = total + (given > free_pages ? given - free_pages : 0);
+    const int64_t missing = (int64_t)total + (given > free_pages ? given - free_pages : 0);
+    p.status[1] = (int)(missing < INT32_MAX ? missing : INT32_MAX);
   }
   for (int r = t; r < p.rows_out; r += kThreads) {
     const Row row = rows[r];

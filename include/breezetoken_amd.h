@@ -389,7 +389,7 @@ int64_t bt_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads,
  * attends the first lens[b] tokens of table row b (clamped to 0 ..
  * pages_per_seq * page_size; none: zeros).  q (batch, heads, head_dim) f32 or
  * bf16, out the same shape f32 or bf16.  head_dim in {64, 128, 256}, heads /
- * kv_heads <= 8, batch <= 4,096, batch * max_tokens < 2^34.  A page may stand in several rows, or twice in
+ * kv_heads <= 8, batch <= 4,096, batch * heads < 2^22, batch * max_tokens < 2^34.  A page may stand in several rows, or twice in
  * one.  `workspace` is scratch for the duration of the call on `stream`: calls
  * that may overlap need one each.  It generalises gqa_decode's split and combine
  * (breezetoken/kernels/cuda/attention.py:54-205). */
@@ -441,7 +441,8 @@ int64_t bt_pages_workspace_bytes(int32_t num_pages, int32_t rows);
  * fresh page in every plane.  table and lens stay as they are and must not
  * overlap the outputs.  status (2,): pages left free, and pages that could not be
  * given (too few pages or entries): those entries are -1, the row's tokens in
- * them lost to the new row, but not to the old one.  No reference counterpart. */
+ * them lost to the new row, but not to the old one; a row counts at most 2^30 /
+ * rows_out.  planes < 2^13.  No reference counterpart. */
 int bt_fork_pages(void* pages, int64_t plane_stride, int64_t page_stride, int32_t planes, int32_t num_pages,
                   int32_t page_size, int32_t token_elems, const int32_t* table, const int32_t* lens,
                   int32_t rows, int32_t pages_per_seq, const int32_t* parent, const int32_t* add,
@@ -470,7 +471,8 @@ int64_t bt_beam_workspace_bytes(int32_t batch, int32_t width, int32_t vocab, int
  * Sums and comparisons are in 64 bits: a beam's candidates go by their logits,
  * equal ones by token, those of two beams by value, equal ones by beam.  A NaN
  * logit counts as -inf; candidates of -inf are chosen only when no others are
- * left.  width and beams <= 64, beams <= width * vocab, vocab <= 2^30.  The reference decodes
+ * left.  width and beams <= 64, beams <= width * vocab, vocab <= 2^30, batch * width
+ * < 2^21.  The reference decodes
  * greedily (breezetoken/model/graph.py:87-91). */
 int bt_beam_select(const void* logits, int32_t dtype, int64_t stride_batch, int64_t stride_beam,
                    const float* scores, int32_t batch, int32_t width, int32_t vocab, int32_t beams,

@@ -44,6 +44,7 @@ ATTN = dict(q=A, q_dtype=0, q_stride=8 * 128, k=A, v=A, sp=16 * 256, st=256, sh=
     (dict(per_seq=0), -22), (dict(ts=3), -22), (dict(batch=0), -22), (dict(heads=9), -22), (dict(kv_heads=0), -22),
     (dict(page=8), -95), (dict(page=48), -95), (dict(page=2048), -95), (dict(dim=96, q_stride=1024), -95),
     (dict(heads=18, q_stride=4096, out_stride=4096), -95), (dict(batch=4097), -95),
+    (dict(batch=4096, heads=2048, kv_heads=2048, q_stride=1 << 18, out_stride=1 << 18), -95),
     (dict(per_seq=1 << 28, ts=1 << 28), -95), (dict(st=1 << 28), -95),
 ])
 def test_attention_refuses(change, code):
@@ -78,6 +79,7 @@ FORK = dict(pages=A, plane=64 * 1024, stride=1024, planes=2, num=64, page=16, el
     (dict(rows=-1), -22), (dict(rows_out=-1), -22), (dict(per_seq=0), -22), (dict(parent=None), -22), (dict(num_keep=2), -22),
     (dict(table_out=None), -22), (dict(table_out=A), -22), (dict(lens_out=None), -22), (dict(lens_out=A), -22),
     (dict(status=None), -22), (dict(plane=2048), -22), (dict(page=24), -95), (dict(per_seq=1 << 30), -95),
+    (dict(planes=8192, plane=1 << 20, stride=1024, num=1024), -95),
     (dict(ws=None), -28), (dict(ws_bytes=64), -28), (dict(ws=A + 4), -28),
 ])
 def test_fork_refuses(change, code):
@@ -104,7 +106,7 @@ BEAM = dict(logits=A, dtype=0, sb=400, sw=100, scores=A, batch=2, width=4, vocab
     (dict(logits=None), -22), (dict(scores=None), -22), (dict(so=None), -22), (dict(po=None), -22), (dict(to=None), -22),
     (dict(dtype=3), -22), (dict(sb=-1), -22), (dict(sw=-100), -22), (dict(batch=0), -22), (dict(width=0), -22),
     (dict(vocab=0), -22), (dict(beams=0), -22), (dict(vocab=1, beams=5), -22), (dict(logits=A + 2), -22), (dict(width=65), -95),
-    (dict(beams=65), -95), (dict(batch=1 << 30), -95), (dict(ws=None), -28), (dict(ws_bytes=8), -28),
+    (dict(beams=65), -95), (dict(batch=1 << 30), -95), (dict(batch=1 << 19), -95), (dict(ws=None), -28), (dict(ws_bytes=8), -28),
 ])
 def test_beam_refuses(change, code):
     assert _lib.lib().bt_beam_select(*{**BEAM, **change}.values()) == code
