@@ -88,8 +88,8 @@ def rope_tables_scaled(cap: int, rope_dim: int, theta: float, method: str, facto
       the factor, a linear ramp between; the tables carry 0.1 ln(factor) + 1."""
     if rope_dim < 2 or rope_dim % 2 or cap < 1:
         raise ValueError(f"invalid rope_dim {rope_dim} or cap {cap}")
-    if not factor >= 1.0 or not theta > 1.0:
-        raise ValueError("factor must be at least 1, theta above 1")
+    if not 1.0 <= factor < math.inf or not 1.0 < theta < math.inf:
+        raise ValueError("factor must be at least 1, theta above 1, both finite")
     half, attn = rope_dim // 2, 1.0
     i = torch.arange(half, dtype=torch.float64)
     inv = theta ** (-i / half)
