@@ -58,25 +58,14 @@ __device__ __forceinline__ int read_entry(const PageOpParams& p, const Row& row,
 
 // Exclusive sum of v over the work-group's threads, and the total.
 __device__ __forceinline__ int block_scan(int v, int& total, int* lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int x = wave_scan(v);
   __syncthreads();  // the sums of the scan before are read
   if (lane == 63) lds[wave] = x;
   __syncthreads();
-  int s = lane < kThreads / 64 ? lds[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < kThreads / 64; o <<= 1) {
-    const int y = __shfl_up(s, o);
-    if (lane >= o) s += y;
-  }
+  const int s = wave_scan(lane < kThreads / 64 ? lds[lane] : 0);
   total = __builtin_amdgcn_readlane(s, kThreads / 64 - 1);
-  const int before = __shfl(s, wave > 0 ? wave - 1 : 0);
-  return x - v + (wave > 0 ? before : 0);
+  return x - v + (wave > 0 ? __builtin_amdgcn_readlane(s, wave - 1) : 0);
 }
 
 // Holders of the pages, 0, 1 or more: bits in LDS, or counts in memory.
@@ -206,6 +195,8 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
   const int t = threadIdx.x;
   Holders<SMALL> h{bits, bits + kSmallPages / 32, l.count};
   Row* rows = SMALL ? small_rows : l.rows;
+  __shared__ int over_sum;
+  if (t == 0) over_sum = 0;
   int total, over = 0;
   if constexpr (SMALL) {
     small_holders(p, h, rows, over);
@@ -246,12 +237,13 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
   int at = block_scan(mine, free_pages, lds);
   for (int i = 0; i < run && first + i < p.num_pages && at < given; ++i)
     if (!h.held((int)first + i)) l.list[at++] = (int)first + i;
-  block_scan(over, total, lds);  // also: the list and the rows are written
+  if (over) atomicAdd(&over_sum, over);
+  __syncthreads();  // also: the list and the rows are written
   if (t == 0) {
     l.copies[0] = p.rows_out;
     l.copies[1] = free_pages;
     p.status[0] = given < free_pages ? free_pages - given : 0;
-    const int64_t missing = (int64_t)total + (given > free_pages ? given - free_pages : 0);
+    const int64_t missing = (int64_t)over_sum + (given > free_pages ? given - free_pages : 0);
     p.status[1] = (int)(missing < INT32_MAX ? missing : INT32_MAX);
   }
   for (int r = t; r < p.rows_out; r += kThreads) {
@@ -278,21 +270,24 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) 
   Holders<SMALL> h{bits, bits + kSmallPages / 32, l.count};
   int over;
   if constexpr (SMALL) small_holders(p, h, small_rows, over);
-  // A thread takes a run of pages: the live ones, then the free places below their
-  // number (holes) and the held pages at or past it (movers), as many.
+  // A thread takes a run of pages.  The free places below the number of live ones (holes) and the
+  // held pages at or past it (movers) are as many; with `before` held pages before page i, i - before
+  // holes come before it, or before - (held pages before page `live`) movers.
+  __shared__ int held_below;
   const int run = (p.num_pages + kThreads - 1) / kThreads;
   const int64_t first = (int64_t)t * run;
   int mine = 0, live;
   for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += h.held((int)first + i);
-  block_scan(mine, live, lds);
-  int holes = 0, movers = 0, total;
-  for (int i = 0; i < run && first + i < p.num_pages; ++i) {
-    const int id = (int)first + i;
-    const bool held = h.held(id);
-    holes += !held && id < live;
-    movers += held && id >= live;
+  int before = block_scan(mine, live, lds);
+  if (live == p.num_pages && t == 0) held_below = live;
+  if (first <= live && live < first + run) {
+    int below = before;
+    for (int i = 0; first + i < live; ++i) below += h.held((int)first + i);
+    held_below = below;
   }
-  int hole = block_scan(holes, total, lds), mover = block_scan(movers, total, lds);
+  __syncthreads();
+  const int total = live - held_below;
+  int hole = (int)first - before, mover = before > held_below ? before - held_below : 0;
   for (int i = 0; i < run && first + i < p.num_pages; ++i) {
     const int id = (int)first + i;
     const bool held = h.held(id);
