@@ -98,14 +98,24 @@ __device__ __forceinline__ uint32_t nth_bound(const uint32_t (&x)[N], int n, uin
   }
   uint32_t lo = ~wave_umax(~least), hi = wave_umax(most);  // `lo` is reached by all
   top = hi;
+  // Quarters: three thresholds a step, whose compares do not wait for one another.
 #pragma unroll 1
-  for (int i = 0; i < 12 && lo < hi; ++i) {
-    const uint32_t mid = lo + (hi - lo + 1) / 2;
-    int reach = 0;
+  for (int i = 0; i < 6 && lo < hi; ++i) {
+    const uint32_t d = hi - lo, t1 = lo + (d >> 2) + 1, t2 = lo + (d >> 1) + 1, t3 = t2 + (d >> 2);
+    int reach1 = 0, reach2 = 0, reach3 = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) reach += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= mid));
-    if (reach >= n) lo = mid;
-    else hi = mid - 1;
+    for (int j = 0; j < N; ++j) {
+      reach1 += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= t1));
+      reach2 += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= t2));
+      reach3 += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= t3));
+    }
+    if (reach2 >= n) {
+      lo = reach3 >= n ? t3 : t2;
+      hi = reach3 >= n ? hi : t3 - 1;
+    } else {
+      hi = reach1 >= n ? t2 - 1 : t1 - 1;
+      lo = reach1 >= n ? t1 : lo;
+    }
   }
   return lo;
 }
