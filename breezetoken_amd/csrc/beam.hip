@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kScanWaves = 4;
 constexpr int kLoads = 4;    // 16-byte loads of a lane per batch
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 16;
 constexpr int kStats = 3;     // of a chunk, behind its keys
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -86,21 +86,27 @@ __device__ __forceinline__ double wave_sum64(double x) {
   return xor_add64<1>(xor_add64<2>(xor_add64<4>(xor_add64<8>(xor_add64<16>(xor_add64<32>(x))))));
 }
 
-// A bound that at least n (1 .. 64) of the wave's 64 N values reach, and few more: the
-// n-th largest to within 2^-12 of the range between the extremes.  `top`: the largest.
+// A bound that at least n (1 .. 64) of the wave's 64 N values reach, and not many more than
+// 5/4 n where they differ by more than `apart`.  0 is no value: with fewer than n others it is the bound.
+// `top`: the largest.
+constexpr uint32_t kBf16Apart = 0xfffe;  // order_bits of bf16 values differ by 2^16
 template <int N>
-__device__ __forceinline__ uint32_t nth_bound(const uint32_t (&x)[N], int n, uint32_t& top) {
-  uint32_t least = x[0], most = x[0];
+__device__ __forceinline__ uint32_t nth_bound(const uint32_t (&x)[N], int n, uint32_t apart, uint32_t& top) {
+  uint32_t least = x[0] - 1, most = x[0];
 #pragma unroll
   for (int j = 1; j < N; ++j) {
-    least = x[j] < least ? x[j] : least;
+    least = x[j] - 1 < least ? x[j] - 1 : least;
     most = x[j] > most ? x[j] : most;
   }
-  uint32_t lo = ~wave_umax(~least), hi = wave_umax(most);  // `lo` is reached by all
+  uint32_t lo = ~wave_umax(~least) + 1, hi = wave_umax(most);  // `lo`: the smallest value
   top = hi;
+  int have = 0;  // reach `lo`
+#pragma unroll
+  for (int j = 0; j < N; ++j) have += __popcll(__builtin_amdgcn_ballot_w64(x[j] >= lo));
+  if (lo == 0 || have < n) return 0;
   // Quarters: three thresholds a step, whose compares do not wait for one another.
 #pragma unroll 1
-  for (int i = 0; i < 6 && lo < hi; ++i) {
+  for (int i = 0; i < 16 && lo < hi && hi - lo > apart && have > n + n / 4; ++i) {
     const uint32_t d = hi - lo, t1 = lo + (d >> 2) + 1, t2 = lo + (d >> 1) + 1, t3 = t2 + (d >> 2);
     int reach1 = 0, reach2 = 0, reach3 = 0;
 #pragma unroll
@@ -112,9 +118,11 @@ __device__ __forceinline__ uint32_t nth_bound(const uint32_t (&x)[N], int n, uin
     if (reach2 >= n) {
       lo = reach3 >= n ? t3 : t2;
       hi = reach3 >= n ? hi : t3 - 1;
+      have = reach3 >= n ? reach3 : reach2;
     } else {
       hi = reach1 >= n ? t2 - 1 : t1 - 1;
       lo = reach1 >= n ? t1 : lo;
+      have = reach1 >= n ? reach1 : have;
     }
   }
   return lo;
@@ -207,7 +215,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
     uint32_t tops[kScanWaves], highest;
 #pragma unroll
     for (int j = 0; j < kScanWaves; ++j) tops[j] = lane_tops[odd][j * 64 + lane];
-    bound = fmaxf(bound, from_order(nth_bound(tops, beams, highest)));
+    bound = fmaxf(bound, from_order(nth_bound(tops, beams, BF16 ? kBf16Apart : 0, highest)));
     top = fmaxf(top, from_order(highest));
     if (v >= v1) continue;
 
@@ -273,11 +281,55 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
   }
 }
 
+// A wave's candidates in LDS, appended as they come.  Where no more fit, and at the end, each lane
+// counts how many are larger than its two (keys differ): its place in order.
+constexpr int kListed = 2 * kMaxBeams;  // the best `beams` and 64 more
+struct Listed {
+  uint64_t* list;
+  int beams, n = 0;
+  uint64_t least = 0;  // the beams-th best when last sorted
+  __device__ __forceinline__ void sort() {
+    const int lane = lane_id();
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t a = lane < n ? list[lane] : 0, b = lane + 64 < n ? list[lane + 64] : 0;
+    int before_a = 0, before_b = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const uint64_t x = list[j];
+      before_a += x > a;
+      before_b += x > b;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane < n && before_a < beams) list[before_a] = a;
+    if (lane + 64 < n && before_b < beams) list[before_b] = b;
+    __builtin_amdgcn_wave_barrier();
+    if (n >= beams) {
+      n = beams;
+      least = list[beams - 1];
+    }
+  }
+  // The lanes' keys for which `want` holds and that may be among the best (0 is none); whether there were any.
+  __device__ __forceinline__ bool add(uint64_t k, bool want) {
+    uint64_t mask = __builtin_amdgcn_ballot_w64(want && k > least);
+    if (n + __popcll(mask) > kListed) {
+      sort();
+      mask = __builtin_amdgcn_ballot_w64(want && k > least);
+    }
+    const int at = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (mask >> lane_id() & 1) list[at] = k;
+    n += __popcll(mask);
+    return mask != 0;
+  }
+};
+
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p) {
+  __shared__ uint64_t lists[kJoinWaves][kListed];
   __shared__ uint64_t row_keys[kMaxBeamWidth * kMaxBeams];
   __shared__ uint64_t order[kMaxBeamWidth * kMaxBeams];
   __shared__ int ranks[kMaxBeamWidth * kMaxBeams];
   __shared__ double row_max[kMaxBeamWidth], row_add[kMaxBeamWidth];
+  __shared__ uint32_t bound_of_all;
+  __shared__ int num_picked;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x, beams = p.beams, chunks = p.chunks;
   for (int w = wave; w < p.width; w += (int)(blockDim.x >> 6)) {
@@ -288,33 +340,29 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     double sum = mine ? stats[chunks + lane] : 0.0;
     const double ref = mine ? stats[2 * chunks + lane] : 0.0;
     const float score = p.scores[(int64_t)b * p.width + w];
-    // The chunks' lists are sorted: their first keys, then the second ones, ... while any is better
-    // than the last taken.  Four places are on their way at a time.
-    Best best;
+    // The chunks' lists are sorted.  Their first keys, or where those are too few the first four, bound which
+    // are looked at, little more than `beams`; the places come one after the other while there are any.  Four
+    // are on their way at a time.
+    Listed best{lists[wave], beams};
+    uint32_t bound = 0;
     bool more = true;
     for (int i0 = 0; i0 < beams && more; i0 += 4) {
       uint64_t k[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) k[i] = mine && i0 + i < beams ? keys[(int64_t)(i0 + i) * chunks + lane] : 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint64_t least = bcast(best.key, beams - 1);
-        uint64_t mask = __builtin_amdgcn_ballot_w64(k[i] > least);
-        if (__popcll(mask) > beams) {  // none below the beams-th largest matters
-          const uint32_t x[1] = {(uint32_t)(k[i] >> 32)};
-          uint32_t unused;
-          const uint32_t bound = nth_bound(x, beams, unused);
-          mask = __builtin_amdgcn_ballot_w64(k[i] > least && (uint32_t)(k[i] >> 32) >= bound);
-        }
-        more = mask != 0;
-        while (mask) {
-          const int l = __builtin_ctzll(mask);
-          mask &= mask - 1;
-          best.insert(bcast(k[i], l));
-        }
+      if (i0 == 0) {
+        const uint32_t x[4] = {(uint32_t)(k[0] >> 32), (uint32_t)(k[1] >> 32), (uint32_t)(k[2] >> 32), (uint32_t)(k[3] >> 32)};
+        const uint32_t first[1] = {x[0]};
+        uint32_t unused;
+        const uint32_t apart = p.bf16 ? kBf16Apart : 0;
+        bound = chunks > beams ? nth_bound(first, beams, apart, unused) : nth_bound(x, beams, apart, unused);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (more) more = best.add(k[i], (uint32_t)(k[i] >> 32) >= bound);
     }
-    if (lane < beams) row_keys[w * beams + lane] = best.key;
+    best.sort();
+    if (lane < beams) row_keys[w * beams + lane] = lane < best.n ? best.list[lane] : 0;
     const double top = (double)wave_fmaxf((float)m);
     // Relative to the row's largest.  The scan's log2(e) is the f32 constant, and so it is here: what that is off by
     // then counts for the distance to the largest only.
@@ -326,8 +374,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     }
   }
   __syncthreads();
-  // Every row's candidates by their value, then each one's rank: how many of the other rows' sorted
-  // lists come before it.
+  // Every row's candidates by their value; where they are many, those that the rows' first four bound (little
+  // more than `beams`); then each one's rank: how many of the other rows' sorted lists come before it.  (us of the
+  // join, all of them ranked / the bounded: 32 rows of 32 96 / 28; 16 of 16 12.5 / 9.1.)
   const int all = p.width * beams;
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const uint64_t key = row_keys[i];
@@ -340,8 +389,29 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     ranks[i] = i % beams;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < all * p.width; i += blockDim.x) {
-    const int c = i / p.width, o = i % p.width, w = c / beams;
+  const bool prune = all * p.width > 2048;
+  int* picked = reinterpret_cast<int*>(lists);
+  static_assert(sizeof(lists) >= sizeof(ranks), "every candidate may be picked");
+  int few = all;
+  if (prune) {
+    if (wave == 0) {
+      uint32_t x[4], unused;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = lane < p.width && j < beams ? (uint32_t)(order[lane * beams + j] >> 32) : 0;
+      const uint32_t bound = nth_bound(x, beams, 0, unused);
+      if (lane == 0) {
+        bound_of_all = bound;
+        num_picked = 0;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < all; i += blockDim.x)
+      if ((uint32_t)(order[i] >> 32) >= bound_of_all) picked[atomicAdd(&num_picked, 1)] = i;
+    __syncthreads();
+    few = num_picked;
+  }
+  for (int i = threadIdx.x; i < few * p.width; i += blockDim.x) {
+    const int j = i / p.width, c = prune ? picked[j] : j, o = i % p.width, w = c / beams;
     const uint64_t mine = order[c];
     if (mine == 0 || o == w) continue;
     const uint64_t least = o < w ? mine : mine + 1;  // equal ones of lower rows come before
@@ -354,9 +424,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     if (lo) atomicAdd(ranks + c, lo);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < all; i += blockDim.x) {
+  for (int j = threadIdx.x; j < few; j += blockDim.x) {
+    const int i = prune ? picked[j] : j, rank = ranks[i];
     const uint64_t mine = order[i];
-    const int rank = ranks[i];
     if (mine && rank < beams) {
       const int64_t out = (int64_t)b * beams + rank;
       const uint64_t u = mine >> 63 ? mine & ~(1ull << 63) : ~mine;

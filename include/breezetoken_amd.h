@@ -468,8 +468,10 @@ int64_t bt_beam_workspace_bytes(int32_t batch, int32_t width, int32_t vocab, int
  * logits (batch, width, vocab) f32 or bf16, unit vocab stride; scores (batch,
  * width) f32.  scores_out (batch, beams) f32, best first; parent_out the row b *
  * width + w that each continues (bt_fork_pages' parent), token_out its token.
- * Sums and comparisons are in 64 bits: a beam's candidates go by their logits,
- * equal ones by token, those of two beams by value, equal ones by beam.  A NaN
+ * A beam's candidates go by their logits, equal ones by token; those of two
+ * beams by value, compared in 64 bits, equal ones by beam.  Exponentials are f32,
+ * added in 64 bits from sixteens on: a beam's log-sum is off by 2^-22 at most, and
+ * candidates of two beams that are nearer than that may come in either order.  A NaN
  * logit counts as -inf; candidates of -inf are chosen only when no others are
  * left.  width and beams <= 64, beams <= width * vocab, vocab <= 2^30, batch * width
  * < 2^21.  The reference decodes

@@ -170,3 +170,42 @@ def test_repeated_and_captured(hip_backend):
 def test_no_searches(hip_backend):
     got = hip_backend.beam_select(torch.zeros(0, 3, 9, device="cuda"), torch.zeros(0, 3, device="cuda"), 2)
     assert [tuple(t.shape) for t in got] == [(0, 2)] * 3
+
+
+def _check_values(be, logits, scores, beams):
+    """The same where candidates of different beams are equal but for the order of their sums' terms.  A row's
+    log-sum is off by e = 2^-22 at most, and beams are ordered by these values: the i-th of them is within e of
+    the i-th exact one, and the exact value of the candidate chosen for it within e of that."""
+    got = be.beam_select(logits.cuda(), scores.cuda(), beams)
+    value = torch.log_softmax(logits.double(), -1) + scores.double()[..., None]
+    value = torch.where(value.isnan(), -math.inf, value)  # a row barred whole
+    B, W, V = value.shape
+    want = value.view(B, -1).sort(descending=True).values[:, :beams]
+    at = (got[1].cpu().long() % W) * V + got[2].cpu().long()
+    mine = value.view(B, -1).gather(1, at)
+    assert all(len(set(x.tolist())) == beams for x in at)
+    fine = want.isfinite()
+    assert torch.equal(mine.isfinite(), fine) and torch.equal(got[0].cpu().isfinite(), fine)
+    assert bool(((mine - want).abs()[fine] <= 2 * 2.0**-22).all())
+    off = (got[0].cpu().double() - mine).abs()
+    assert bool((off[fine] <= mine.abs()[fine] * orc.F32 + 2.0**-22).all())
+
+
+@pytest.mark.parametrize("W,beams,V", [(64, 64, 300), (40, 64, 70), (20, 20, 3000), (33, 1, 500)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_equal_candidates(hip_backend, W, beams, V, dtype):
+    """Logits of few values and equal scores: more candidates reach any bound than lists hold."""
+    g = torch.Generator().manual_seed(W)
+    logits = torch.randint(0, 2, (2, W, V), generator=g).to(dtype)
+    logits[1] = 0.5
+    _check(hip_backend, logits[1:], torch.zeros(1, W), beams)
+    _check_values(hip_backend, logits, torch.zeros(2, W), beams)
+    logits[0, : W // 2] = -math.inf  # barred whole: they come last
+    logits[0, W // 2 :, 3:] = -math.inf
+    _check_values(hip_backend, logits, torch.zeros(2, W), beams)
+
+
+@pytest.mark.parametrize("W,beams", [(32, 32), (64, 64), (48, 10), (2, 64)])
+def test_wide_searches(hip_backend, W, beams):
+    _check(hip_backend, *_case(2, W, 20000, torch.bfloat16, seed=W), beams)
+    _check(hip_backend, *_case(2, W, 9001, seed=W), beams)
