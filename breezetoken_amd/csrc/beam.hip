@@ -325,7 +325,7 @@ struct Listed {
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p) {
   __shared__ uint64_t lists[kJoinWaves][kListed];
   __shared__ uint64_t row_keys[kMaxBeamWidth * kMaxBeams];
-  __shared__ uint64_t order[kMaxBeamWidth * kMaxBeams];
+  __shared__ uint64_t order[kMaxBeamWidth * (kMaxBeams | 1)];  // rows of beams | 1: an odd pitch keeps rows' places in banks of their own
   __shared__ int ranks[kMaxBeamWidth * kMaxBeams];
   __shared__ double row_max[kMaxBeamWidth], row_add[kMaxBeamWidth];
   __shared__ uint32_t bound_of_all;
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
   // Every row's candidates by their value; where they are many, those that the rows' first four bound (little
   // more than `beams`); then each one's rank: how many of the other rows' sorted lists come before it.  (us of the
   // join, all of them ranked / the bounded: 32 rows of 32 96 / 28; 16 of 16 12.5 / 9.1.)
-  const int all = p.width * beams;
+  const int all = p.width * beams, pitch = beams | 1;
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const uint64_t key = row_keys[i];
     const double top = row_max[i / beams], add = row_add[i / beams];
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     double v = x == top && x != -(double)INFINITY ? add : x - top + add;
     v = v != v ? -(double)INFINITY : v + 0.0;
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    order[i] = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;  // 0: no candidate, behind every other
+    order[i / beams * pitch + i % beams] = key ? (u >> 63 ? ~u : u | 1ull << 63) : 0;  // 0: no candidate, behind every other
     ranks[i] = i % beams;
   }
   __syncthreads();
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     if (wave == 0) {
       uint32_t x[4], unused;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = lane < p.width && j < beams ? (uint32_t)(order[lane * beams + j] >> 32) : 0;
+      for (int j = 0; j < 4; ++j) x[j] = lane < p.width && j < beams ? (uint32_t)(order[lane * pitch + j] >> 32) : 0;
       const uint32_t bound = nth_bound(x, beams, 0, unused);
       if (lane == 0) {
         bound_of_all = bound;
@@ -406,19 +406,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     }
     __syncthreads();
     for (int i = threadIdx.x; i < all; i += blockDim.x)
-      if ((uint32_t)(order[i] >> 32) >= bound_of_all) picked[atomicAdd(&num_picked, 1)] = i;
+      if ((uint32_t)(order[i / beams * pitch + i % beams] >> 32) >= bound_of_all) picked[atomicAdd(&num_picked, 1)] = i;
     __syncthreads();
     few = num_picked;
   }
   for (int i = threadIdx.x; i < few * p.width; i += blockDim.x) {
-    const int j = i / p.width, c = prune ? picked[j] : j, o = i % p.width, w = c / beams;
-    const uint64_t mine = order[c];
+    const int j = i % few, c = prune ? picked[j] : j, o = i / few, w = c / beams;
+    const uint64_t mine = order[w * pitch + c % beams];
     if (mine == 0 || o == w) continue;
     const uint64_t least = o < w ? mine : mine + 1;  // equal ones of lower rows come before
     int lo = 0, hi = beams;  // places of row o that come before: [0, lo), from hi on none
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (order[o * beams + mid] >= least) lo = mid + 1;
+      if (order[o * pitch + mid] >= least) lo = mid + 1;
       else hi = mid;
     }
     if (lo) atomicAdd(ranks + c, lo);
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
   __syncthreads();
   for (int j = threadIdx.x; j < few; j += blockDim.x) {
     const int i = prune ? picked[j] : j, rank = ranks[i];
-    const uint64_t mine = order[i];
+    const uint64_t mine = order[i / beams * pitch + i % beams];
     if (mine && rank < beams) {
       const int64_t out = (int64_t)b * beams + rank;
       const uint64_t u = mine >> 63 ? mine & ~(1ull << 63) : ~mine;
