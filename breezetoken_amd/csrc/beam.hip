@@ -19,11 +19,11 @@
 // sixteens, then in 64.  A second kernel, a work-group per batch item, joins the chunks
 // of a row and then the rows.
 //
-// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 20 us, of which its loads alone
-// 13 (4.9 TB/s); exponentials and sums, the bound, and the selection add 2 to 3 each, since
+// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 19 us, of which its loads alone
+// 13 (4.9 TB/s); exponentials and sums, the bound, and the selection add about 2 each, since
 // a wave asks for its next logits when it is done with these.  With twice the registers
 // and the next ones asked for before the work it took 22: every row is on its way at once
-// then.  The join takes 6.5, a chain of dependent steps in a work-group per batch item.
+// then.  The join takes 5.5, a chain of dependent steps in a work-group per batch item.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -376,7 +376,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
   __syncthreads();
   // Every row's candidates by their value; where they are many, those that the rows' first four bound (little
   // more than `beams`); then each one's rank: how many of the other rows' sorted lists come before it.  (us of the
-  // join, all of them ranked / the bounded: 32 rows of 32 96 / 28; 16 of 16 12.5 / 9.1.)
+  // join, all ranked / the bounded: 8 rows of 8 candidates 5.6 / 6.6, 16 of 8 7.7 / 7.7, 16 of 16 10.5 / 9.1, 32
+  // of 32 40 / 19.)
   const int all = p.width * beams, pitch = beams | 1;
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const uint64_t key = row_keys[i];
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
 // Chunks of a row, at most 64, and their size (whole wave loads): 4,096 waves in all where
 // the rows are long enough, each at least 2,048 logits (a bf16 batch), whole work-groups.  us a call, bf16: 128
 // rows of 248,320 26, with 2,048 waves 30; 128 rows of 32,000 13.7 with 1,000 logits a wave,
-// 12.3 with 2,000.
+// 12.3 with 2,000 (before the join's last changes, on both sides).
 int beam_chunks(int batch, int width, int vocab, int* size) {
   const int64_t rows = (int64_t)batch * width;
   int64_t want = (4096 + rows - 1) / rows;
