@@ -6,11 +6,14 @@
 //
 // A plan (who holds each page, which pages go where) and the copies it asks for.
 // The copies are bound by memory.  The plan is a chain of short steps over little
-// data, bound by latency and launches: up to kSmallPages pages, kSmallRows rows
-// and kSmallCells table entries one work-group makes all of it, holders as two
-// bits of each page in LDS (held; held twice), rows in LDS, counts by prefix sums
-// over its threads.  Larger caches count holders in memory with the whole chip;
-// the steps between stay with one work-group.
+// data, bound by latency and launches: in small caches (is_small) one work-group makes
+// all of it, holders as two bits of each page in LDS (held; held twice), rows in LDS, a
+// page's place from the held pages before its word of bits.  Larger ones count holders
+// in memory with the whole chip; the steps between stay with one work-group.
+//
+// us, plan + copies: fork of 4 rows in 320 pages 4.8 + 2.5, of 128 rows in 2,048 pages of
+// 12 planes 8.2 + 8.0 (31 MB); compaction of 300 pages 4.3 + 6.6, of 2,048 (395 MB read
+// and written) 7.0 + 82, 4.8 TB/s, a large copy's rate.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
@@ -20,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kAhead = 8;  // table entries a thread has on their way at a time
-constexpr int kSmallPages = 1 << 18, kSmallRows = 2048, kSmallCells = 1 << 16;
+constexpr int kSmallPages = 1 << 18, kSmallRows = 2048;  // what LDS holds
 
 // A row of the result: where it comes from, its tokens, the entries it will have,
 // and the rank among the pages given of its first one.
@@ -92,6 +95,22 @@ struct Holders {
     else return count[id] > 1;
   }
 };
+
+// Held pages before each word of a small cache's bits, by the whole work-group; all of them in `held`.
+__device__ __forceinline__ void words_before(const PageOpParams& p, const Holders<true>& h, int* before, int& held, int* lds) {
+  const int words = (p.num_pages + 31) / 32, run = (words + kThreads - 1) / kThreads, first = (int)threadIdx.x * run;
+  int mine = 0;
+  for (int i = first; i < first + run && i < words; ++i) mine += __popc(h.once[i]);
+  int at = block_scan(mine, held, lds);
+  for (int i = first; i < first + run && i < words; ++i) {
+    before[i] = at;
+    at += __popc(h.once[i]);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ int held_before(const Holders<true>& h, const int* before, int id) {
+  return before[id >> 5] + __popc(h.once[id >> 5] & ((1u << (id & 31)) - 1));
+}
 
 // A thread's walk over the (row, column) cells t, t + kThreads, ...: one work-group does
 // all of a small cache's, so a division for each would be most of the work.
@@ -189,6 +208,7 @@ __global__ void pages_count_kernel(PageOpParams p) {
 template <bool SMALL>
 __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
   __shared__ uint32_t bits[SMALL ? 2 * (kSmallPages / 32) : 1];
+  __shared__ int before[SMALL ? kSmallPages / 32 : 1];
   __shared__ Row small_rows[SMALL ? kSmallRows : 1];
   __shared__ int lds[kThreads / 64];
   const Layout l = layout_of(p);
@@ -228,15 +248,25 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
     if (r < p.rows_out) rows[r] = row;
     given += total;
   }
-  // Free pages in order, as many as are given: a thread takes a run of pages.
-  const int run = (p.num_pages + kThreads - 1) / kThreads;
-  const int64_t first = (int64_t)t * run;
-  int mine = 0;
-  for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += !h.held((int)first + i);
+  // Free pages in order, as many as are given.
   int free_pages;
-  int at = block_scan(mine, free_pages, lds);
-  for (int i = 0; i < run && first + i < p.num_pages && at < given; ++i)
-    if (!h.held((int)first + i)) l.list[at++] = (int)first + i;
+  if constexpr (SMALL) {
+    int held;
+    words_before(p, h, before, held, lds);
+    free_pages = p.num_pages - held;
+    for (int base = 0; base < p.num_pages && base - before[base >> 5] < given; base += kThreads) {
+      const int id = base + t, rank = id < p.num_pages ? id - held_before(h, before, id) : given;
+      if (rank < given && !h.held(id)) l.list[rank] = id;
+    }
+  } else {  // a thread takes a run of pages
+    const int run = (p.num_pages + kThreads - 1) / kThreads;
+    const int64_t first = (int64_t)t * run;
+    int mine = 0;
+    for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += !h.held((int)first + i);
+    int at = block_scan(mine, free_pages, lds);
+    for (int i = 0; i < run && first + i < p.num_pages && at < given; ++i)
+      if (!h.held((int)first + i)) l.list[at++] = (int)first + i;
+  }
   if (over) atomicAdd(&over_sum, over);
   __syncthreads();  // also: the list and the rows are written
   if (t == 0) {
@@ -263,6 +293,7 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(PageOpParams p) {
 template <bool SMALL>
 __global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) {
   __shared__ uint32_t bits[SMALL ? 2 * (kSmallPages / 32) : 1];
+  __shared__ int before[SMALL ? kSmallPages / 32 : 1];
   __shared__ Row small_rows[SMALL ? kSmallRows : 1];
   __shared__ int lds[kThreads / 64];
   const Layout l = layout_of(p);
@@ -270,31 +301,40 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) 
   Holders<SMALL> h{bits, bits + kSmallPages / 32, l.count};
   int over;
   if constexpr (SMALL) small_holders(p, h, small_rows, over);
-  // A thread takes a run of pages.  The free places below the number of live ones (holes) and the
-  // held pages at or past it (movers) are as many; with `before` held pages before page i, i - before
-  // holes come before it, or before - (held pages before page `live`) movers.
-  __shared__ int held_below;
-  const int run = (p.num_pages + kThreads - 1) / kThreads;
-  const int64_t first = (int64_t)t * run;
-  int mine = 0, live;
-  for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += h.held((int)first + i);
-  int before = block_scan(mine, live, lds);
-  if (live == p.num_pages && t == 0) held_below = live;
-  if (first <= live && live < first + run) {
-    int below = before;
-    for (int i = 0; first + i < live; ++i) below += h.held((int)first + i);
-    held_below = below;
-  }
-  __syncthreads();
-  const int total = live - held_below;
-  int hole = (int)first - before, mover = before > held_below ? before - held_below : 0;
-  for (int i = 0; i < run && first + i < p.num_pages; ++i) {
-    const int id = (int)first + i;
-    const bool held = h.held(id);
-    if (held && id >= live) l.copies[4 + 4 * (int64_t)mover++] = id;
+  // The free places below the number of live pages (holes) and the held pages at or past it (movers)
+  // are as many; with n held pages before page i, i - n holes come before it, or n - (held pages
+  // before page `live`) movers.
+  int live, below;  // held pages before page `live`
+  auto place = [&](int id, bool held, int n) {
+    if (held && id >= live) l.copies[4 + 4 * (int64_t)(n - below)] = id;
     else p.where[id] = held ? id : -1;
-    if (!held && id < live) l.list[hole++] = id;
+    if (!held && id < live) l.list[id - n] = id;
+  };
+  if constexpr (SMALL) {
+    words_before(p, h, before, live, lds);
+    below = live < p.num_pages ? held_before(h, before, live) : live;
+    for (int id = t; id < p.num_pages; id += kThreads) place(id, h.held(id), held_before(h, before, id));
+  } else {  // a thread takes a run of pages
+    __shared__ int below_live;
+    const int run = (p.num_pages + kThreads - 1) / kThreads;
+    const int64_t first = (int64_t)t * run;
+    int mine = 0;
+    for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += h.held((int)first + i);
+    int n = block_scan(mine, live, lds);
+    if (live == p.num_pages && t == 0) below_live = live;
+    if (first <= live && live < first + run) {
+      below_live = n;
+      for (int i = 0; first + i < live; ++i) below_live += h.held((int)first + i);
+    }
+    __syncthreads();
+    below = below_live;
+    for (int i = 0; i < run && first + i < p.num_pages; ++i) {
+      const bool held = h.held((int)first + i);
+      place((int)first + i, held, n);
+      n += held;
+    }
   }
+  const int total = live - below;
   __syncthreads();
   for (int m = t; m < total; m += kThreads) {
     int* copy = l.copies + 4 + 4 * (int64_t)m;
@@ -363,9 +403,13 @@ __global__ __launch_bounds__(kApplyThreads) void pages_apply_kernel(PageOpParams
   p.table_out[i] = id;
 }
 
+// One work-group reads 2^16 table entries in 22 us; the whole chip needs two more launches, and the one
+// work-group of its other steps time for each page.  us of a fork (a compaction), one work-group / the chip: 128
+// rows of 128 entries in 8,192 pages 13.5 (13.3) / 17.7 (20.7), of 256 18.9 (17.6) / 18.4 (20.4), of 512 29.6
+// (26.8) / 20.6 (21.4); 256 of 512 in 32,768 pages 49 (52) / 37 (76); 1,024 of 512 in 2^18 169 (339) / 184 (565).
 bool is_small(const PageOpParams& p) {
   return p.num_pages <= kSmallPages && p.rows_out <= kSmallRows &&
-         (int64_t)p.rows_out * p.pages_per_seq + p.num_keep <= kSmallCells;
+         (int64_t)p.rows_out * p.pages_per_seq + p.num_keep <= (1 << 15) + 2 * p.num_pages;
 }
 
 dim3 per_cell(int64_t n) { return dim3((unsigned)((n + 255) / 256)); }

@@ -212,3 +212,30 @@ def test_captured(hip_backend):
         assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)) and torch.equal(p.cpu(), want[3])
         want = orc.compact(pages, table, lens)
         assert all(torch.equal(a.cpu(), b) for a, b in zip(got2, want)) and torch.equal(p2.cpu(), want[3])
+
+
+@pytest.mark.parametrize("N,rows,per_row", [(700, 100, 600), (700, 50, 600), (5000, 70, 600), (40000, 300, 350), (270000, 3, 40)])
+def test_many_entries_in_few_pages_and_few_in_many(hip_backend, N, rows, per_row):
+    """Both sides of where the whole chip counts holders: entries against pages."""
+    page = 16
+    g = torch.Generator().manual_seed(N + rows)
+    pages, table, lens = _cache(rows, N, page, 8, 2, per_row * page - 200, per_row, seed=rows, prefix=3)
+    lens[::7] = 0
+    if N < 1000:  # leave pages free: rows of ten ids between them
+        table = table % 10 + 3
+        table[:, 2] = 690
+    parent = torch.randint(-1, rows, (rows,), generator=g, dtype=torch.int32)
+    add = torch.randint(0, 40, (rows,), generator=g, dtype=torch.int32)
+    keep = torch.tensor([N - 1, 5, -1, N], dtype=torch.int32)
+    _fork(hip_backend, pages, table, lens, parent, add, keep)
+    _compact(hip_backend, pages, table, lens, keep)
+
+
+def test_compact_pages_of_one_word_and_of_all_words(hip_backend):
+    """Held pages at the words' ends: 31, 32, 33, the last, and none in between."""
+    for N in (31, 32, 33, 64, 1000, 33000):
+        pages = torch.arange(2 * N, dtype=torch.float32).view(2, N, 1, 1).expand(2, N, 16, 8).to(torch.bfloat16).contiguous()
+        ids = sorted({i for i in (0, 30, 31, 32, 33, 63, N - 2, N - 1) if 0 <= i < N})
+        table = torch.tensor([ids[::-1]], dtype=torch.int32)
+        _compact(hip_backend, pages, table, _ints(16 * len(ids)))
+        _fork(hip_backend, pages, table, _ints(16 * len(ids) - 5), _ints(0, 0), _ints(1, 1))
