@@ -6,9 +6,12 @@
 //
 // A table entry outside [0, num_pages) holds no keys.
 //
-// Bound by the stream of K and V.  The batch's tiles (16 tokens each, never
-// across a page) are numbered through, sequence after sequence, and every
-// work-group of a kv head takes an equal run of them, whatever sequences it
+// Bound by the stream of K and V: 32 sequences of 256 to 32,768 tokens, H = 8, Hkv = 2,
+// D = 256 (454 MB), take 71 us, 6.35 TB/s, and the combine 4.7; one of 131,072, H = 16, 44
+// and 4.6; 24 of 1,800 to 3,000, H = 32, Hkv = 8, D = 128, 40 and 4.7.
+//
+// The batch's tiles (16 tokens each, never across a page) are numbered through, sequence
+// after sequence, and every work-group of a kv head takes an equal run of them, whatever sequences it
 // falls into: all CUs stream the same number of bytes for any mix of lengths,
 // with no plan, no host lengths and no rounds of work-groups.  A run that covers
 // a sequence writes its result; the parts of a sequence cut by a run's end go to
@@ -507,11 +510,16 @@ int paged_runs(int batch, int kv_heads, int head_dim, int64_t max_tokens, int nu
   const int64_t most = (int64_t)batch * ((max_tokens + 15) / 16);  // tiles of the largest call
   // Short tables: a work-group per sequence, which writes its result, and no combine.
   // us a graph node (issued one by one), whole sequences / runs, D = 256, Hkv = 2: one
-  // sequence of 128 tokens 7.3 (9.4) / 8.6 (13.5), 256 8.8 (9.6) / 8.6 (13.6), 512 11.9
-  // (11.7) / 8.7 (13.4); 128 sequences of 256 13.7 / 19.1; D = 128, Hkv = 8: one of 512
-  // 9.1 (9.6) / 8.5 (13.7), 1,024 12.8 (12.7) / 8.9 (13.7), 128 of 512 58 / 62; D = 64,
-  // Hkv = 4: one of 512 7.1 (9.6) / 7.3 (13.7), 1,024 10.2 (10.1) / 7.4 (13.7).
+  // sequence of 128 tokens 6.4 (9.6) / 8.8 (13.2), 256 7.6 (9.6) / 8.8 (13.3), 512 10.7
+  // (10.6) / 8.8 (13.3); D = 128, Hkv = 8: one of 512 7.4 (9.7) / 7.7 (13.1), 1,024 10.9
+  // (11.0) / 7.7 (13.2); D = 64, Hkv = 4: one of 512 5.8 (9.8) / 7.1 (13.1).
   if (max_tokens <= 512 && max_tokens * head_dim <= 65536) return 0;
+  // Where sequences fill the chip, longer ones too: every run would end some of them.  us,
+  // all full / lengths uniform / their logarithms uniform, whole sequences and then runs:
+  // 128 of up to 1,024, D = 256, Hkv = 2 42 / 30 / 23, 48 / 36 / 28; 300 of up to 1,024, D =
+  // 128, Hkv = 8 201 / 112 / 45, 215 / 120 / 59; 128 of up to 512, D = 64 13 / 10 / 8, 16 /
+  // 18 / 18; 128 of up to 2,048, D = 256 82 / 52 / 43, 89 / 52 / 34 (the longest one counts).
+  if (max_tokens <= 1024 && (int64_t)batch * kv_heads >= num_cus) return 0;
   // One work-group a CU: two (D = 128, 64) keep more requests on their way, and the HBM
   // serves them less well.  us, one / two: H = 32, Hkv = 8, D = 128, 32 x 8,000 tokens
   // 166 / 172, 24 x 3,000 53 / 55, one of 131,072 89 / 91; H = 16, Hkv = 2 26 / 34; D =

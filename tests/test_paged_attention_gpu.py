@@ -368,6 +368,25 @@ def test_threads_call_at_once(hip_backend):
     assert not wrong
 
 
+@pytest.mark.parametrize("batch", [65, 512, 513, 700, 4096])
+def test_runs_over_many_sequences_of_long_tables(hip_backend, batch):
+    """Room for 2,048 tokens a row: runs for any number of sequences, windows of their lengths past the eighth."""
+    g = torch.Generator().manual_seed(batch)
+    lens = [int(x) for x in torch.exp(torch.rand(batch, generator=g) * 4.0) - 1.0]
+    lens[batch // 2] = 2048
+    lens[batch - 1] = 700
+    _check(hip_backend, *_case(lens, 2, 1, 64, 16, per_row=128, seed=batch))
+
+
+@pytest.mark.parametrize("H,G,D,batch", [(8, 2, 256, 128), (8, 2, 256, 127), (32, 8, 128, 32), (15, 5, 64, 60)])
+def test_sequences_that_fill_the_chip(hip_backend, H, G, D, batch):
+    """A work-group per sequence up to 1,024 tokens, and a batch that is one short of that."""
+    g = torch.Generator().manual_seed(batch)
+    lens = [int(x) for x in torch.exp(torch.rand(batch, generator=g) * 6.9)]
+    lens[0], lens[5], lens[batch - 1] = 1024, 0, 1023
+    _check(hip_backend, *_case(lens, H, G, D, 64, per_row=16, seed=batch))
+
+
 def test_no_sequences(hip_backend):
     q, k, v, table, lens = _case([3], 8, 2, 128, 16)
     got = hip_backend.attention_paged(q[:0].cuda(), k.cuda(), v.cuda(), table[:0].cuda(), lens[:0].cuda(), 0.1)
