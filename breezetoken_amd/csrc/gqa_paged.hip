@@ -26,10 +26,10 @@
 // on the current one, also across the end of a sequence, so the merge and the
 // next sequence's queries hide behind the stream.
 //
-// The MFMA takes K as it is and the query heads of the group as columns.  f32
-// queries and probabilities enter as sums of bf16 terms in further columns (and,
-// for 5 to 8 heads, a second MFMA): three terms hold all 24 bits where the output
-// is f32, two leave 2^-16 where it is rounded to bf16 (2^-8).
+// The MFMA takes K as it is and the query heads of the group as columns.  Scaled
+// queries and probabilities enter as sums of three bf16 terms, which hold all 24 bits
+// of them, in further columns (and, for 5 to 8 heads, a second MFMA).  Two terms, for 5
+// to 8 heads where the output is rounded to bf16 (2^-8), leave 2^-16 (launch_mode).
 #include "bt_common.h"
 #include "bt_decode.h"
 #include "bt_kernels.h"
@@ -82,7 +82,7 @@ constexpr int kKeptWindows = 8;  // in LDS: 512 sequences; further windows load 
 
 // WHOLE: work-group w takes sequence w, numbered alone; two of them fit a CU below D =
 // 256 (128 registers).  Runs have a CU each (paged_runs) and take 130 to 195.
-template <int GMAX, int D, bool QBF16, bool F32OUT, bool WHOLE>
+template <int GMAX, int D, bool QBF16, int TERMS, bool WHOLE>
 __global__ __launch_bounds__(kWaves * 64, WHOLE && D < 256 ? 4 : 2) void gqa_paged_kernel(PagedDecodeParams p) {
   constexpr int kThreads = kWaves * 64;
   constexpr int kSteps = D / 32;
@@ -93,8 +93,7 @@ __global__ __launch_bounds__(kWaves * 64, WHOLE && D < 256 ? 4 : 2) void gqa_pag
   constexpr int kLoads = kTileBytes / 1024;  // 1 KiB wave loads per K or V tile
   constexpr int kRowsPerLoad = 1024 / kRowBytes;
   constexpr int kGroups = 16 / GMAX;                  // column groups
-  constexpr int kTerms = F32OUT ? 3 : 2;
-  constexpr bool kSecond = kTerms > kGroups;          // the third term in an MFMA of its own
+  constexpr bool kSecond = TERMS > kGroups;           // the third term in an MFMA of its own
   constexpr int kMoStride = D + 4;
   static_assert(kSteps == kLoads && kSteps <= kWaves, "one wave per d-step builds Q^T");
 
@@ -188,14 +187,14 @@ __global__ __launch_bounds__(kWaves * 64, WHOLE && D < 256 ? 4 : 2) void gqa_pag
   // A value's terms as packed bf16: this lane's, and (second) the third one for the first columns.
   const uint32_t keep0 = term == 0 && col_head < G ? 0xffffffffu : 0u;
   const uint32_t keep1 = term == 1 && col_head < G ? 0xffffffffu : 0u;
-  const uint32_t keep2 = !kSecond && kTerms == 3 && term == 2 && col_head < G ? 0xffffffffu : 0u;
+  const uint32_t keep2 = !kSecond && TERMS == 3 && term == 2 && col_head < G ? 0xffffffffu : 0u;
   auto terms2 = [&](float a, float b, uint32_t& second) -> uint32_t {
     const uint32_t h = f32x2_to_bf16x2_bits(a, b);
     a -= __uint_as_float(h << 16);
     b -= __uint_as_float(h & 0xffff0000u);
     const uint32_t m = f32x2_to_bf16x2_bits(a, b);
     uint32_t r = (h & keep0) | (m & keep1);
-    if constexpr (kTerms == 3) {
+    if constexpr (TERMS == 3) {
       const uint32_t l = f32x2_to_bf16x2_bits(a - __uint_as_float(m << 16), b - __uint_as_float(m & 0xffff0000u));
       if constexpr (kSecond) second = l & keep0;
       else r |= l & keep2;
@@ -486,17 +485,26 @@ __global__ __launch_bounds__(kWaves * 64, WHOLE && D < 256 ? 4 : 2) void gqa_pag
   }
 }
 
+template <int GMAX, int D, int TERMS, bool WHOLE>
+hipError_t launch_terms(const PagedDecodeParams& p, hipStream_t stream) {
+  const dim3 grid((WHOLE ? p.batch : p.runs) * p.kv_heads), block(kWaves * 64);
+  if (p.q_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, TERMS, WHOLE>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, TERMS, WHOLE>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
+// Two terms only where a third would take an MFMA of its own and the result is rounded to
+// bf16: 300 of 100,000 results then round to the other side, 50 with three (and 60 in plain
+// f32 torch operations).  us, two / three terms, bf16 out, 8 heads a kv head: one sequence
+// of 131,072, D = 256 47.2 / 48.3; 16 of 4,000 28.3 / 29.5; one of 500, D = 128, whole 7.4 /
+// 8.2; 512 of 500, D = 64 11.4 / 11.8.  Up to 4 heads (24 of 2,400, D = 128 42.2 / 42.5; 512
+// of 500, D = 64 22.0 / 22.1) the columns are there.
 template <int GMAX, int D, bool WHOLE>
 hipError_t launch_mode(const PagedDecodeParams& p, hipStream_t stream) {
-  const dim3 grid((WHOLE ? p.batch : p.runs) * p.kv_heads), block(kWaves * 64);
-  if (p.q_bf16) {
-    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, false, WHOLE>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, true, true, WHOLE>), grid, block, 0, stream, p);
-  } else {
-    if (p.out_bf16) hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, false, WHOLE>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_paged_kernel<GMAX, D, false, true, WHOLE>), grid, block, 0, stream, p);
+  if constexpr (GMAX > 4) {
+    if (p.out_bf16) return launch_terms<GMAX, D, 2, WHOLE>(p, stream);
   }
-  return hipGetLastError();
+  return launch_terms<GMAX, D, 3, WHOLE>(p, stream);
 }
 
 template <int GMAX, int D>
