@@ -85,7 +85,9 @@ def rope_tables_scaled(cap: int, rope_dim: int, theta: float, method: str, facto
       is slowed by the factor and the fastest keeps its rate;
     * ``yarn`` (Peng et al., 2023): pairs that turn at least 32 times over the
       trained context keep their rate, those that turn at most once are slowed by
-      the factor, a linear ramp between; the tables carry 0.1 ln(factor) + 1."""
+      the factor, between them a ramp linear in the pair's number, from the last
+      whole one before the first border to the first behind the other; the tables
+      carry 0.1 ln(factor) + 1."""
     if rope_dim < 2 or rope_dim % 2 or cap < 1:
         raise ValueError(f"invalid rope_dim {rope_dim} or cap {cap}")
     if not 1.0 <= factor < math.inf or not 1.0 < theta < math.inf:
@@ -102,8 +104,8 @@ def rope_tables_scaled(cap: int, rope_dim: int, theta: float, method: str, facto
         if not trained or trained < 1:
             raise ValueError("yarn needs the trained context length")
         low, high = (half * math.log(trained / (2 * math.pi * turns)) / math.log(theta) for turns in (32, 1))
-        low, high = max(0, math.floor(low)), min(half - 1, math.ceil(high))
-        slow = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        low, high = math.floor(low), math.ceil(high)  # either may lie outside the pairs
+        slow = ((i - low) / (high - low)).clamp(0, 1)
         inv = inv / factor * slow + inv * (1 - slow)
         attn = 0.1 * math.log(factor) + 1.0
     else:
