@@ -1081,9 +1081,10 @@ class HipBackend:
 
         logits (B, W, V) f32 or bf16, scores (B, W) f32 -> (scores (B, beams) f32, best
         first, parent (B, beams) int32, the row b * W + w each continues, token (B,
-        beams) int32).  Compared in 64 bits, over log-sums that are off by 2^-22 at most;
-        ties go to the lower beam, then to the lower token.  A barred token has the logit -inf (NaN counts as that); a beam
-        that has ended keeps its score with one logit of 0 and -inf elsewhere."""
+        beams) int32).  Compared in 64 bits, over log-sums that are off by 2^-21 at most;
+        ties go to the lower beam, then to the lower token.  A barred token has the
+        logit -inf (NaN counts as that); a beam that has ended keeps its score with one
+        logit of 0 and -inf elsewhere."""
         shape = logits.shape
         if len(shape) != 3 or scores.shape != shape[:2]:
             raise RuntimeError("beam_select expects logits (B, W, V) and scores (B, W)")

@@ -12,14 +12,22 @@
 // The work-group's lanes exchange the largest of theirs: the beams-th largest of these
 // 256 values bounds which logits can be chosen, so of 16,384 logits little more than
 // `beams` are looked at; they enter the wave's best, sorted 64-bit keys (order of the
-// logit, ~token) across its lanes.  The largest is the exponentials' reference: c, its
-// product with log2(e) rounded to a whole number, so that each is one fused
-// multiply-add x log2(e) - c, exact to 2^-24 of itself, and one v_exp, and sums of
-// any lanes, waves and chunks add after a power of two.  They are added in 32 bits by
-// sixteens, then in 64.  A second kernel, a work-group per batch item, joins the chunks
-// of a row and then the rows.
+// logit, ~token) across its lanes.  The exponentials' reference is a whole number: c, the
+// largest's product with log2(e) rounded, so that each is one fused multiply-add
+// x log2(e) - c and one v_exp, and sums of any lanes, waves and chunks add after a power
+// of two.
 //
-// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 19 us, of which its loads alone
+// The multiply-add rounds to 2^-24 of its result, so far below the reference terms would be
+// off by 2^-20, and alike where they are equal.  So c is that of a lane's sixteen logits,
+// whose terms weigh the less the more they are off; what is missing from the float over
+// log2(e) multiplies their sum.  Eights are added in 32 bits (three levels), the rest in
+// 64.  A log-sum is off by 2^-21 at most: 2^-23 of v_exp, 3 x 2^-24 of the eights, and under 2.5 x
+// 2^-24 of the exponents and the factor; 0.7 x 2^-22 was the most seen over rows of equal
+// logits far below one peak, 1.6 to 2.2 with the work-group's largest as the only reference
+// and eights added one by one (2% of the time: 128 rows of bf16 24.7 / 25.1 us, f32 33.5 / 33.7).
+// A second kernel, a work-group per batch item, joins the chunks of a row and then the rows.
+//
+// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 20 us, of which its loads alone
 // 13 (4.9 TB/s); exponentials and sums, the bound, and the selection add about 2 each, since
 // a wave asks for its next logits when it is done with these.  With twice the registers
 // and the next ones asked for before the work it took 22: every row is on its way at once
@@ -36,6 +44,8 @@ constexpr int kLoads = 4;    // 16-byte loads of a lane per batch
 constexpr int kJoinWaves = 16;
 constexpr int kStats = 3;     // of a chunk, behind its keys
 constexpr float kLog2e = 1.44269504088896340736f;
+// 2^(n kRest) = 1 + n kLog2eRest, kRest what is missing from 1 of the float over log2(e).
+constexpr float kLog2eRest = (float)((1.44269504088896340736 / (double)kLog2e - 1.0) * 0.69314718055994530942);
 
 // Order-preserving bits of a float (-0 as +0), and back.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -225,10 +235,20 @@ __global__ __launch_bounds__(kScanWaves * 64) void beam_scan_kernel(BeamParams p
 #pragma unroll
     for (int i = 0; i < kBatches; ++i) {
       if (v + i * kBatch >= v1) break;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) part[e & 3] += fast_exp2(fmaf(logit(raw[i], e), kLog2e, -ref));
-      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+      for (int e0 = 0; e0 < kElems; e0 += 2 * kGroup) {
+        const int g = (i * kElems + e0) / kGroup;
+        const float own = fmaxf(rintf(fmaxf(most[g], most[g + 1]) * kLog2e), ref - 256.f);
+        float part[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[kGroup];
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) x[e] = fast_exp2(fmaf(logit(raw[i], e0 + h * kGroup + e), kLog2e, -own));
+          part[h] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        }
+        sum += ((double)part[0] + (double)part[1]) * (double)(fast_exp2(own - ref) * fmaf(own, kLog2eRest, 1.f));
+      }
     }
 
     uint64_t least = bcast(best.key, beams - 1);
@@ -364,9 +384,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(BeamParams p
     best.sort();
     if (lane < beams) row_keys[w * beams + lane] = lane < best.n ? best.list[lane] : 0;
     const double top = (double)wave_fmaxf((float)m);
-    // Relative to the row's largest.  The scan's log2(e) is the f32 constant, and so it is here: what that is off by
-    // then counts for the distance to the largest only.
-    const double power = ref != ref ? (m - top) * 1.4426950408889634 : ref - top * (double)kLog2e;
+    // Relative to the row's largest.
+    const double power = ref != ref ? (m - top) * 1.4426950408889634 : ref - top * 1.4426950408889634;
     sum = wave_sum64(sum == 0.0 || (ref != ref && m == top) ? sum : sum * exp2(power));
     if (lane == 0) {
       row_max[w] = top;

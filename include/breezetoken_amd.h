@@ -470,8 +470,9 @@ int64_t bt_beam_workspace_bytes(int32_t batch, int32_t width, int32_t vocab, int
  * width + w that each continues (bt_fork_pages' parent), token_out its token.
  * A beam's candidates go by their logits, equal ones by token; those of two
  * beams by value, compared in 64 bits, equal ones by beam.  Exponentials are f32,
- * added in 64 bits from sixteens on: a beam's log-sum is off by 2^-22 at most, and
- * candidates of two beams that are nearer than that may come in either order.  A NaN
+ * eights of them added in 32 bits, the rest in 64: a beam's log-sum is off by 2^-21
+ * at most, and candidates of two beams that are nearer than 2^-20 may come in either
+ * order.  A NaN
  * logit counts as -inf; candidates of -inf are chosen only when no others are
  * left.  width and beams <= 64, beams <= width * vocab, vocab <= 2^30, batch * width
  * < 2^21.  The reference decodes

@@ -1,0 +1,74 @@
+"""Beam selection's log-sums where the mass lies far below the largest logit."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+# A logit's exponential is taken relative to the largest of sixteen.  The exponent's rounding moves the sixteen's
+# sum by 2^-24 at most: terms of 2^-a of the largest are off by 2^-24 a ln 2, and weigh 15 x 2^-a together.  The
+# missing part of log2(e) moves it by a third of that, v_exp by 2^-23, three f32 additions by 2^-24 each, the
+# factor's rounding by 2^-24; all further sums are in 64 bits.  7.3 x 2^-24 together.
+LOG_SUM = 2.0**-21
+
+
+def _flat_rows(top, low, V, dtype):
+    """Rows of one logit `top` and V - 1 of `low`; the log-sum less `top`, in 64 bits."""
+    top, low = top.to(dtype), low.to(dtype)
+    x = low.cuda()[:, None].expand(len(top), V).clone()
+    x[:, V // 3] = top.cuda()
+    return x, torch.log1p((V - 1) * torch.exp(low.double() - top.double()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [32000, 248320])
+@pytest.mark.parametrize("batch", [1, 17])  # 17: so many rows that one work-group, and one reference, takes a whole one
+@pytest.mark.parametrize("near,far", [(6.0, 9.0), (9.0, 11.0), (11.1, 12.4)])
+def test_a_peak_above_equal_logits(hip_backend, dtype, V, batch, near, far):
+    g = torch.Generator().manual_seed(int(far * 10))
+    W = 64
+    top = torch.rand(W, generator=g) * 40 - 20
+    low = top - near - (far - near) * torch.rand(W, generator=g)
+    top[0], low[0] = 7.30921, -3.6139622
+    x, less = _flat_rows(top, low, V, dtype)
+    # Scores that leave of each row's best candidate little but its sum's error, a step apart: the order is theirs.
+    scores = (less + torch.arange(W) * 2.0**-19).float()
+    exact = scores.double() - less
+    logits = x.expand(batch, W, V)
+    got, parent, token = (t.cpu() for t in hip_backend.beam_select(logits, scores.cuda().expand(batch, W).contiguous(), W))
+    assert bool((token == V // 3).all())
+    rows = parent.long() % W
+    assert float((got.double() - exact[rows]).abs().max()) <= LOG_SUM
+    # Exact values are at least 2^-19 - 2^-20 apart (the scores' own rounding), both sums off by LOG_SUM at most.
+    assert bool((rows == torch.arange(W - 1, -1, -1)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch", [1, 17])
+def test_shapes_of_mass(hip_backend, dtype, batch):
+    """Steps of equal logits, spread ones, and sixteens that hold one large logit each."""
+    V, W = 50000, 6
+    g = torch.Generator().manual_seed(5)
+    x = torch.empty(W, V)
+    x[0] = torch.linspace(-14, 0, V)
+    x[1] = -torch.arange(V).float().remainder(16)
+    x[2] = -11.37
+    x[2, ::16] = 3.21
+    x[3] = torch.randn(V, generator=g) * 5
+    x[4] = torch.randn(V, generator=g).abs() * -3 - 80
+    x[5] = -4000.3
+    x[5, 7] = -3990.1
+    x = x.to(dtype)
+    less = torch.logsumexp(x.double(), 1) - x.double().max(1).values
+    scores = less.float()
+    logits = x.cuda().expand(batch, W, V)
+    for w in range(W):  # one row live at a time
+        s = torch.full((batch, W), -math.inf)
+        s[:, w] = scores[w]
+        got, parent, _ = (t.cpu() for t in hip_backend.beam_select(logits, s.cuda(), 1))
+        assert bool((parent[:, 0] == torch.arange(batch) * W + w).all())
+        assert float((got.double() - (scores[w].double() - less[w])).abs().max()) <= LOG_SUM

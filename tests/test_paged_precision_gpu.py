@@ -24,3 +24,12 @@ def test_bf16_results_of_small_groups(hip_backend, H, G, D, q_dtype, per_row):
     lens = [40 + 7 * (b % 11) for b in range(60)]
     got, want, tol = _run(hip_backend, rows(lens, H, G, D, 16, per_row, q_dtype), torch.bfloat16)
     assert int((~rounds_to(got, want, tol)).sum()) == 0
+
+
+@pytest.mark.parametrize("per_row", [16, 128])
+@pytest.mark.parametrize("H,G,D", [(8, 2, 256), (16, 4, 128), (15, 5, 64), (7, 1, 128), (16, 2, 256), (5, 1, 64), (6, 1, 128)])
+@pytest.mark.parametrize("q_dtype,spread", [(torch.float32, 1.0), (torch.float32, 6.0), (torch.bfloat16, 1.0)])
+def test_f32_results(hip_backend, H, G, D, q_dtype, spread, per_row):
+    q, *rest = rows([2, 5, 17, 40, 130, 200], H, G, D, 16, per_row, seed=H)
+    got, want, tol = _run(hip_backend, [(q * spread).to(q_dtype), *rest], torch.float32)
+    assert float(((got.double() - want).abs() / tol).max()) <= 1.0
