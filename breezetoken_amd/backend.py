@@ -1027,11 +1027,13 @@ class HipBackend:
         its pages shared, and has room for ``add`` more tokens ((rows,) int32 or one
         number): free pages, lowest first, and a copy of the last page where that is
         partly filled and held by another row or by ``keep`` (int32 page ids that must
-        stay).  A page no new row holds and ``keep`` does not name is free: sequences
+        stay); every row that will write to such a page gets one, the last of them too.  A page no new row holds and ``keep`` does not name is free: sequences
         end by having no child.  Returns (table, lens, status): new tensors, lens
         without the added tokens, status (2,) int32 = pages left free and pages that
         could not be given -- their entries are -1, and the old table still names
-        what the new rows would lose, so the step can be taken again."""
+        what the new rows would lose, so the step can be taken again: from the rows
+        that this call continued and those whose pages ``keep`` named.  The pages of
+        the others were free to it, and may hold copies by then."""
         args, before, kept = self._page_args(pages, table, lens, keep)
         rows_in, per_seq = before[2], before[3]
         if parent is None:

@@ -438,11 +438,13 @@ int64_t bt_pages_workspace_bytes(int32_t num_pages, int32_t rows);
  * (add NULL: none) hold pages, the further ones -1: pages no new row holds, nor
  * `keep` (num_keep ids), lowest first, in row order.  Where add[i] > 0 and the
  * last page is partly filled and held more than once, its tokens are copied to a
- * fresh page in every plane.  table and lens stay as they are and must not
+ * fresh page in every plane, for each such row.  table and lens stay as they are and must not
  * overlap the outputs.  status (2,): pages left free, and pages that could not be
  * given (too few pages or entries): those entries are -1, the row's tokens in
- * them lost to the new row, but not to the old one; a row counts at most 2^30 /
- * rows_out.  planes < 2^13.  No reference counterpart. */
+ * them lost to the new row, but not to the old one.  Old rows that no new row
+ * continues are free, here too: copies may have been written to their pages, so that
+ * the call can be repeated from the continued rows only, and from those whose pages
+ * `keep` named.  A row counts at most 2^30 / rows_out missing pages.  planes < 2^13.  No reference counterpart. */
 int bt_fork_pages(void* pages, int64_t plane_stride, int64_t page_stride, int32_t planes, int32_t num_pages,
                   int32_t page_size, int32_t token_elems, const int32_t* table, const int32_t* lens,
                   int32_t rows, int32_t pages_per_seq, const int32_t* parent, const int32_t* add,
