@@ -321,13 +321,13 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(PageOpParams p) 
     int mine = 0;
     for (int i = 0; i < run && first + i < p.num_pages; ++i) mine += h.held((int)first + i);
     int n = block_scan(mine, live, lds);
-    if (live == p.num_pages && t == 0) below_live = live;
-    if (first <= live && live < first + run) {
-      below_live = n;
-      for (int i = 0; first + i < live; ++i) below_live += h.held((int)first + i);
+    if (live < p.num_pages && first <= live && live < first + run) {  // one thread
+      int m = n;
+      for (int i = 0; first + i < live; ++i) m += h.held((int)first + i);
+      below_live = m;
     }
     __syncthreads();
-    below = below_live;
+    below = live < p.num_pages ? below_live : live;
     for (int i = 0; i < run && first + i < p.num_pages; ++i) {
       const bool held = h.held((int)first + i);
       place((int)first + i, held, n);
