@@ -159,6 +159,7 @@ int bt_attn_prep_paged(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, i
   if (rc) return rc;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) return BT_ENOTSUP;
   if ((int64_t)tokens * (heads + 2 * (int64_t)kv_heads) > INT32_MAX / 64) return BT_ENOTSUP;
+  if (row > INT32_MAX) return BT_ENOTSUP;  // a token's values are numbered in 32 bits
   bt::PagedPrepParams p{};
   p.x = qkv;
   p.x_bf16 = qkv_dtype == BT_DTYPE_BF16;

@@ -414,7 +414,8 @@ int bt_gqa_decode_paged(const void* q, int32_t q_dtype, int64_t q_stride_seq, co
  * (rows NULL: row t), rounded to bf16; a row outside [0, table_rows), a
  * position outside the row or an entry outside the cache writes neither.  Two
  * tokens of one call must not name the same slot: which one it then holds is
- * not defined.  head_dim in {64, 128, 256, 512}. */
+ * not defined.  head_dim in {64, 128, 256, 512}; a row holds at most 2^31 - 1
+ * values. */
 int bt_attn_prep_paged(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, int32_t tokens, int32_t heads,
                        int32_t kv_heads, int32_t head_dim, int32_t gated, const float* q_norm,
                        const float* k_norm, float eps, const float* cos, const float* sin, int32_t rope_dim,
