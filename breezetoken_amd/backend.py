@@ -101,7 +101,7 @@ def rope_tables_scaled(cap: int, rope_dim: int, theta: float, method: str, facto
         if rope_dim > 2:
             inv = (theta * factor ** (rope_dim / (rope_dim - 2))) ** (-i / half)
     elif method == "yarn":
-        if not trained or trained < 1:
+        if trained is None or not 1 <= trained < math.inf:
             raise ValueError("yarn needs the trained context length")
         low, high = (half * math.log(trained / (2 * math.pi * turns)) / math.log(theta) for turns in (32, 1))
         low, high = math.floor(low), math.ceil(high)  # either may lie outside the pairs

@@ -49,3 +49,9 @@ def test_yarn_tables(rope_dim, theta, factor, trained):
             assert abs(float(back[i]) - plain / factor) <= 2.0**-22
         else:
             assert plain / factor - 2.0**-22 <= float(back[i]) <= plain + 2.0**-22
+
+
+@pytest.mark.parametrize("trained", [None, 0, -1, math.inf, math.nan])
+def test_trained_lengths_that_are_none(trained):
+    with pytest.raises(ValueError, match="trained context"):
+        rope_tables_scaled(16, 64, 1.0e4, "yarn", 8.0, trained, "cpu")
