@@ -27,11 +27,11 @@
 // and eights added one by one (2% of the time: 128 rows of bf16 24.7 / 25.1 us, f32 33.5 / 33.7).
 // A second kernel, a work-group per batch item, joins the chunks of a row and then the rows.
 //
-// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 20 us, of which its loads alone
-// 13 (4.9 TB/s); exponentials and sums, the bound, and the selection add about 2 each, since
+// 128 rows of 248,320 bf16 logits (64 MB): the scan takes 20.5 us, of which its loads alone
+// 13 (4.9 TB/s); exponentials and sums, the bound, and the selection add 2 to 3 each, since
 // a wave asks for its next logits when it is done with these.  With twice the registers
 // and the next ones asked for before the work it took 22: every row is on its way at once
-// then.  The join takes 5.5, a chain of dependent steps in a work-group per batch item.
+// then.  The join takes 5.6, a chain of dependent steps in a work-group per batch item.
 #include "bt_common.h"
 #include "bt_kernels.h"
 
