@@ -72,3 +72,45 @@ def test_shapes_of_mass(hip_backend, dtype, batch):
         got, parent, _ = (t.cpu() for t in hip_backend.beam_select(logits, s.cuda(), 1))
         assert bool((parent[:, 0] == torch.arange(batch) * W + w).all())
         assert float((got.double() - (scores[w].double() - less[w])).abs().max()) <= LOG_SUM
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch", [1, 17])
+@pytest.mark.parametrize("order", [0, 1, 2])
+def test_stretches_of_different_size(hip_backend, dtype, batch, order):
+    """Rows of stretches that no common reference suits: near 0, near the largest, thousands below it, barred,
+    not a number; a stretch's logits within three of one another.  Largest logits up to 4,096 and past it."""
+    V, W, piece = 70001, 64, 1777
+    g = torch.Generator().manual_seed(order)
+    levels = torch.tensor([0.0, 11.0, -300.0, 4.0, -5000.0, -math.inf, math.nan, 7.5, -90.0])
+    x = torch.randn(W, V, generator=g).clamp(-3, 3)
+    for at in range(0, V, piece):
+        x[:, at : at + piece] += levels[torch.randint(0, len(levels), (W, 1), generator=g)]
+    x += torch.tensor([0.0, 4080.0, -3900.0, 30000.0, -6000.0, 1.0e6])[torch.arange(W) % 6][:, None]
+    if order == 1:
+        x = x.sort(dim=1).values  # NaN last
+    elif order == 2:
+        x = x.nan_to_num(-math.inf, None, -math.inf).sort(dim=1, descending=True).values
+    x = x.to(dtype)
+    clean = torch.where(x.isnan(), -math.inf, x.double())
+    top = clean.max(1).values
+    less = torch.log(torch.exp(clean - top[:, None]).sum(1))
+    scores = less.float() - 60 * torch.arange(W)  # every row's best candidates before the next row's
+    exact = scores.double() - less
+    got, parent, token = (t.cpu() for t in hip_backend.beam_select(x.cuda().expand(batch, W, V),
+                                                                   scores.cuda().expand(batch, W).contiguous(), 64))
+    first = clean.argmax(1)  # the lowest of equal ones
+    for b in range(batch):
+        assert int(parent[b, 0]) == b * W and int(token[b, 0]) == int(first[0])
+        assert abs(float(got[b, 0]) - float(exact[0])) <= LOG_SUM
+        # The order inside the row, and values: 64 candidates of row 0.
+        best = torch.sort(clean[0], descending=True, stable=True)
+        assert torch.equal(token[b].long(), best.indices[:64]) and bool((parent[b] == b * W).all())
+        want = best.values[:64] - top[0] + exact[0]
+        assert float((got[b].double() - want).abs().max()) <= LOG_SUM + float(want.abs().max()) * 2.0**-24
+    for w in range(1, W, 5):
+        s = torch.full((batch, W), -math.inf)
+        s[:, w] = less[w].float()
+        got, parent, token = (t.cpu() for t in hip_backend.beam_select(x.cuda().expand(batch, W, V), s.cuda(), 1))
+        assert bool((token == first[w]).all()) and bool((parent[:, 0] == torch.arange(batch) * W + w).all())
+        assert float((got.double() - (less[w].float().double() - less[w])).abs().max()) <= LOG_SUM
