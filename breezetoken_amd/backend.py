@@ -836,17 +836,14 @@ class HipBackend:
     # input where one fits (1.2 us; torch.empty with a type and device 1.7).
     def _run(self, name: str, *args) -> None:
         """Launch on this backend's device, whichever is current."""
-        rc = self._on_device(getattr(self._lib, name), *args, _stream(self._dev))
+        fn, dev = getattr(self._lib, name), self._dev
+        if torch._C._cuda_getDevice() == dev.index:
+            rc = fn(*args, _stream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, _stream(dev))
         if rc:
             check(name, rc)
-
-    def _on_device(self, fn, *args) -> int:
-        """A C entry point that looks at the current device, on this backend's."""
-        dev = self._dev
-        if torch._C._cuda_getDevice() == dev.index:
-            return fn(*args)
-        with torch.cuda.device(dev):
-            return fn(*args)
 
     def _ints(self, name: str, t: torch.Tensor, n: int) -> int:
         """Address of a contiguous int32 device tensor of n values."""
@@ -910,11 +907,13 @@ class HipBackend:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        out = torch.empty_like(q, dtype=out_dtype)
         if batch == 0:
-            return out
-        nbytes = self._on_device(self._lib.bt_paged_workspace_bytes, batch, heads, groups, dim,
-                                 min(per_seq * size, 0x7FFFFFFF))
+            return torch.empty_like(q, dtype=out_dtype)
+        if torch._C._cuda_getDevice() != self._dev.index:  # the workspace follows from the current device's CUs
+            with torch.cuda.device(self._dev):
+                return self.attention_paged(q, k, v, table, lens, scale, out_dtype)
+        out = torch.empty_like(q, dtype=out_dtype)
+        nbytes = self._lib.bt_paged_workspace_bytes(batch, heads, groups, dim, min(per_seq * size, 0x7FFFFFFF))
         ws = lens.new_empty(nbytes >> 2) if nbytes else None
         row = heads * dim
         self._run("bt_gqa_decode_paged", q.data_ptr(), q_code, row, k.data_ptr(), v.data_ptr(), sp, st, sh, pages, size,
