@@ -14,8 +14,8 @@
 // for two sets of 16, leaves one wave a SIMD and was slower by half.)  S^T = K Q^T
 // leaves the scores of a row in four lanes, which then are, rounded, the operand of
 // O^T += V^T P^T as they lie; V is read transposed from LDS.  f32 queries and the
-// probabilities enter as sums of bf16 terms (three hold all 24 bits, two 16, for results
-// rounded to bf16).  The next tile's scores are worked out beside this one's softmax.
+// probabilities enter as sums of three bf16 terms, which hold all 24 bits of them.  The
+// next tile's scores are worked out beside this one's softmax.
 //
 // The tiles of the batch are dealt out by the work-groups themselves, from the lengths, in
 // parts of one sequence each, or in equal runs where sequences are many; parts are joined by
@@ -78,8 +78,14 @@ __device__ __forceinline__ void mfma_settle(floatx4 (&acc)[N]) {
 // 54.1 (32 sequences of 256 to 32,768 tokens, D = 128; in runs across sequences 63 and 56).
 constexpr int kGroups = 2;
 
-// QT: bf16 terms of a query (3: f32, 1: bf16 as it is), PT: of a probability.
-template <int D, int QT, int PT>
+// bf16 terms of a probability, also where the result is rounded to bf16: with two, 3,101 of the 1,572,864 results of 24
+// sequences of 1,800 to 3,000 tokens (16 drafts, H = 32, Hkv = 8, D = 128) fall to the wrong side of that rounding, with
+// three 560 (777 in plain f32 torch operations).  us, two / three: that case 52.6 / 53.3, 32 of 500 19.1 / 19.5, and where
+// products are what counts, 64 drafts of 16 heads behind 32,768, bf16 queries, 64 / 73.
+constexpr int kTerms = 3;
+
+// QT: bf16 terms of a query (3: f32, 1: bf16 as it is).
+template <int D, int QT>
 __global__ __launch_bounds__(kWaves * 64, kGroups) void gqa_tree_kernel(TreeParams p) {
   constexpr int kSteps = D / 32;
   constexpr int kDT = D / 16;
@@ -402,9 +408,9 @@ __global__ __launch_bounds__(kWaves * 64, kGroups) void gqa_tree_kernel(TreePara
     // One step's work before its products: the probabilities' terms, in stages between the products of
     // the next tile's scores, which the matrix unit works on meanwhile (behind the last tile: of zeros;
     // a branch around them costs more).
-    u32x4 pop[PT];
+    u32x4 pop[kTerms];
     auto advance = [&](const unsigned char* kt, const Scores& s) -> Scores {
-      constexpr int kStages = 2 + PT;
+      constexpr int kStages = 2 + kTerms;
       float v[8], sum = 0.f;
       auto stage = [&](int i) {
         if (i < 2) {
@@ -503,7 +509,7 @@ __global__ __launch_bounds__(kWaves * 64, kGroups) void gqa_tree_kernel(TreePara
 #pragma unroll
       for (int dt = 0; dt < kDT; dt += 2) {
 #pragma unroll
-        for (int term = 0; term < PT; ++term)
+        for (int term = 0; term < kTerms; ++term)
 #pragma unroll
           for (int i = 0; i < 2; ++i) oacc[dt + i] = mfma16(vop[(dt + i) % kAhead], as_bf16x8(pop[term]), oacc[dt + i]);
 #pragma unroll
@@ -698,19 +704,18 @@ __global__ __launch_bounds__(T) void tree_join_kernel(TreeParams p) {
   }
 }
 
-template <int D, int QT, int PT>
+template <int D, int QT>
 hipError_t launch_terms(TreeParams p, hipStream_t stream) {
   const int pairs = (p.runs ? p.runs + p.batch : p.batch) * p.kv_heads;
   const dim3 grid((unsigned)((pairs + 7) / 8 * 8 * p.row_blocks));
   const size_t lds = p.runs && p.batch > 64 ? (size_t)p.batch * 4 : 0;
-  hipLaunchKernelGGL((gqa_tree_kernel<D, QT, PT>), grid, dim3(kWaves * 64), lds, stream, p);
+  hipLaunchKernelGGL((gqa_tree_kernel<D, QT>), grid, dim3(kWaves * 64), lds, stream, p);
   return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_dim(const TreeParams& p, hipStream_t stream) {
-  if (p.q_bf16) return p.out_bf16 ? launch_terms<D, 1, 2>(p, stream) : launch_terms<D, 1, 3>(p, stream);
-  return p.out_bf16 ? launch_terms<D, 3, 2>(p, stream) : launch_terms<D, 3, 3>(p, stream);
+  return p.q_bf16 ? launch_terms<D, 1>(p, stream) : launch_terms<D, 3>(p, stream);
 }
 
 }  // namespace
