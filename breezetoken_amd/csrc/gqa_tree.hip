@@ -642,12 +642,11 @@ __global__ __launch_bounds__(T) void tree_join_kernel(TreeParams p) {
   const int64_t slot = (int64_t)head * (p.runs + p.batch) + p.part_base[b];
   float m = -INFINITY, l = 0.f;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
+  // Also with a weight of zero: a part's values that are not finite stay that in the result.
   auto add = [&](float top, float x, const float4& v) {
     const float wgt = fast_exp2(x - (top == -INFINITY ? 0.f : top));
-    if (wgt != 0.f) {
-      l += wgt;
-      acc.x += wgt * v.x; acc.y += wgt * v.y; acc.z += wgt * v.z; acc.w += wgt * v.w;
-    }
+    l += wgt;
+    acc.x += wgt * v.x; acc.y += wgt * v.y; acc.z += wgt * v.z; acc.w += wgt * v.w;
   };
   for (int s = count == 1 ? count : part; s < count; s += kAhead * S) {
     float x[kAhead];
@@ -668,7 +667,8 @@ __global__ __launch_bounds__(T) void tree_join_kernel(TreeParams p) {
     l *= old;
     acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(top, x[i], v[i]);
+    for (int i = 0; i < kAhead; ++i)
+      if (s + i * S < count) add(top, x[i], v[i]);
     m = top;
   }
   // The groups' sums, the upper half's into the lower's until one is left.
