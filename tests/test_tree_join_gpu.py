@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_tree_attention_gpu import _case, _run
+from tests.test_tree_attention_gpu import _case, _check, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,12 @@ def test_a_cached_value_without_a_number_counts_whatever_its_parts_weight(hip_ba
     assert not got[b, :, : H // G, 7].isfinite().any()
     got[b, :, : H // G, 7] = 0
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("batch,short,longest", [(64, 20, 9000), (64, 300, 9000), (130, 40, 5000), (31, 40, 12000), (3, 10, 30000), (2, 10, 60000)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_one_long_sequence_among_short_ones(hip_backend, batch, short, longest, D):
+    """Most of the parts are one sequence's."""
+    lens = [short] * batch
+    lens[batch // 3] = longest
+    _check(hip_backend, *_case(lens, 2, 2, 1, D, 64))
