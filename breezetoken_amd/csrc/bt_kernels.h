@@ -505,10 +505,12 @@ struct SelectParams {
   const int32_t* lens;
   int32_t batch, heads, kv_heads, group, head_dim;
   int32_t count;
-  double* score;        // (batch, kv_heads, pages_per_seq)
+  double* score;        // (batch, kv_heads, pages_per_seq), or null where there is nothing to choose: needs_scores()
   int32_t* chosen;      // (batch, kv_heads, count) page ids, -1 behind them
   int32_t* chosen_len;  // (batch,) tokens in them
 };
+// Rows of up to `count` pages keep all of them, and one page is the last one.
+inline bool needs_scores(int32_t pages_per_seq, int32_t count) { return count > 1 && pages_per_seq > count; }
 hipError_t launch_select_pages(const SelectParams& p, hipStream_t stream);
 
 struct PagedPrepParams {

@@ -288,7 +288,7 @@ int bt_key_bounds(const void* k, int64_t stride_page, int64_t stride_tok, int64_
 }
 
 int64_t bt_select_workspace_bytes(int32_t batch, int32_t kv_heads, int32_t pages_per_seq, int32_t count) {
-  if (batch < 1 || kv_heads < 1 || pages_per_seq < 1 || pages_per_seq <= count) return 0;
+  if (batch < 1 || kv_heads < 1 || pages_per_seq < 1 || !bt::needs_scores(pages_per_seq, count)) return 0;
   return align256((int64_t)batch * kv_heads * pages_per_seq * 8);
 }
 
@@ -336,7 +336,7 @@ int bt_select_pages(const void* q, int32_t q_dtype, int64_t q_stride_seq, const 
   if (rc) return rc;
   const int64_t bytes = bt_select_workspace_bytes(batch, kv_heads, pages_per_seq, count);
   if (bytes && (!workspace || !aligned16(workspace) || workspace_bytes < bytes)) return BT_ENOSPC;
-  p.score = static_cast<double*>(workspace);
+  p.score = bytes ? static_cast<double*>(workspace) : nullptr;
   p.chosen = chosen;
   p.chosen_len = chosen_lens;
   return hip_rc(bt::launch_select_pages(p, (hipStream_t)stream));
@@ -377,7 +377,7 @@ int bt_gqa_decode_sparse(const void* q, int32_t q_dtype, int64_t q_stride_seq, c
   const SparseWorkspace ws = sparse_workspace(batch, heads, kv_heads, head_dim, pages_per_seq, page_size, count);
   if (!workspace || !aligned16(workspace) || workspace_bytes < ws.bytes) return BT_ENOSPC;
   char* at = static_cast<char*>(workspace);
-  p.score = reinterpret_cast<double*>(at);
+  p.score = ws.chosen ? reinterpret_cast<double*>(at) : nullptr;
   p.chosen = reinterpret_cast<int32_t*>(at + ws.chosen);
   p.chosen_len = reinterpret_cast<int32_t*>(at + ws.lens);
   bt::PagedDecodeParams d{};

@@ -341,12 +341,12 @@ __global__ __launch_bounds__(T) void page_choose_kernel(SelectParams p, int per)
   __shared__ double list[kListed];
   __shared__ int list_at[kListed];
   const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  // `per` consecutive entries a thread, asked for before the row's length is there.  (Where every row keeps
-  // all its pages there are no scores, and no place for them.)
+  // `per` consecutive entries a thread, asked for before the row's length is there.  (Where there are no
+  // scores there is no place for them.)
   const int first = tid * per;
   double x[kPerThread] = {};
   int id[kPerThread] = {};
-  if (p.pg.pages_per_seq > p.count) {
+  if (p.score) {
     const double* score = p.score + ((int64_t)b * p.kv_heads + kvh) * p.pg.pages_per_seq;
     const int32_t* table = p.pg.table + (int64_t)b * p.pg.table_stride;
 #pragma unroll
@@ -610,7 +610,7 @@ hipError_t launch_key_bounds(const BoundsParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_select_pages(const SelectParams& p, hipStream_t stream) {
-  if (p.pg.pages_per_seq > p.count) {
+  if (p.score) {
     hipError_t e;
     switch (p.head_dim) {
       case 64: e = launch_score_dim<64>(p, stream); break;
