@@ -1176,9 +1176,9 @@ class HipBackend:
         last page, and those of the others whose keys' bounds (``key_bounds``) allow the
         largest product with a query of its group.  Rows of up to ``count`` pages attend all of
         them; the last page's bounds are not read, so those of a page are needed from its
-        last token on.  A page's score is the largest over the group's heads of sum_d
-        max(q_d * low_d, q_d * high_d), in 64 bits; ties go to the earlier page.  ``scale``
-        must be positive."""
+        last token on.  A page's score is the largest over the group's heads of sum_d q_d *
+        (high_d where q_d > 0, else low_d), in 64 bits; ties go to the earlier page, and pages
+        with a channel that holds no number come last.  ``scale`` must be positive."""
         if q.ndim != 3:
             raise RuntimeError("sparse attention expects q (B, H, D)")
         batch, heads, dim = q.shape

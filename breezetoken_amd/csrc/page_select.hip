@@ -2,8 +2,8 @@
 // choice of pages by them.
 //
 //   low / high[page, g, d] = min / max over the page's tokens of k[token, g, d]   (NaN keys left out)
-//   score[b, g, e] = max over the group's heads h of sum_d max(q_hd low_d, q_hd high_d)
-//     >= every product of those heads with a key of page table[b, e]
+//   score[b, g, e] = max over the group's heads h of sum_d q_hd (q_hd > 0 ? high_d : low_d)
+//     >= every product of those heads with a key of page table[b, e]; -inf where a channel has no number (low > high)
 //   chosen[b, g]: the last page, and the best count - 1 of the others (ties: the lower
 //     entry), in the order of the table
 //

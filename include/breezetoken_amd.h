@@ -446,7 +446,7 @@ int bt_accept_drafts(void* pages, int64_t plane_stride, int64_t page_stride, int
  * tokens below lens[b]: bounds (num_pages, kv_heads, 2, head_dim) bf16, contiguous,
  * 16-byte aligned.  Further pages' bounds stay as they are.  A partly filled page that
  * several rows have as the same entry gets the bounds of the row with most tokens.  NaN
- * keys are left out.  batch <= 4,096.  No reference counterpart. */
+ * keys are left out (a channel of nothing else: low = inf, high = -inf).  batch <= 4,096.  No reference counterpart. */
 int bt_key_bounds(const void* k, int64_t stride_page, int64_t stride_tok, int64_t stride_head,
                   int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_stride,
                   int32_t pages_per_seq, const int32_t* lens, const int32_t* first, int32_t batch,
@@ -457,10 +457,12 @@ int64_t bt_select_workspace_bytes(int32_t batch, int32_t kv_heads, int32_t pages
 
 /* The pages that a new token of each sequence attends, kv head by kv head: the row's
  * last page and, of the others, the count - 1 with the largest score -- of the group's
- * heads the largest sum over d of max(q_d * low_d, q_d * high_d), which no product of a
- * head with one of the page's keys exceeds (the product with 1 / sqrt(D) or any other
- * positive scale follows the same order).  Scores are sums in 64 bits; ties go to the
- * earlier page; a score that is not a number and a page outside the cache count as -inf.
+ * heads the largest sum over d of q_d * b_d, b_d being high_d where q_d > 0 and low_d
+ * elsewhere, which no product of a head with one of the page's keys exceeds (the product
+ * with 1 / sqrt(D) or any other positive scale follows the same order).  Scores are sums
+ * in 64 bits; ties go to the earlier page; a head's sum that is not a number and a page
+ * outside the cache count as -inf.  So does a page with a channel that holds no number, whose
+ * bounds bt_key_bounds leaves as low = inf, high = -inf.
  * chosen (batch, kv_heads, count) int32: page ids in the row's order, -1 behind them; a
  * row of up to count pages keeps all of them.  chosen_lens (batch,): tokens in them.
  * What bt_gqa_decode_sparse attends.  The last page's bounds are not read.  No reference

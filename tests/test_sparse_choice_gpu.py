@@ -5,7 +5,6 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests import drafts_oracle as drafts
 from tests.test_sparse_attention_gpu import _attend, _case, _choice, _stale
 
 pytestmark = pytest.mark.gpu
@@ -20,3 +19,32 @@ def test_the_last_page_alone(hip_backend, pages):
     _attend(hip_backend, q, k, v, limit, table, lens, 1)
     got = hip_backend.select_pages(q.cuda(), torch.full_like(limit, float("nan")).cuda(), table.cuda(), lens.cuda(), 1, 16)
     assert torch.equal(got[0].cpu(), ref[0]) and torch.equal(got[1].cpu(), ref[1])
+
+
+@pytest.mark.parametrize("H,G", [(4, 2), (16, 2)])
+@pytest.mark.parametrize("zero", [False, True])
+def test_pages_with_a_channel_without_a_number_come_last(hip_backend, H, G, zero):
+    """Whatever their other channels say: the bounds of such a channel are low = inf, high = -inf, and its term -inf,
+    or, with a query of zero there, no number."""
+    page, count = 16, 4
+    q, k, v, table, lens = _case([160], H, G, 64, page)
+    k[table[0, 3].long(), :, :, 2] = 1e4  # would be the best
+    q[..., 2] = 1.0
+    k[table[0, 3].long(), :, 0, 5] = float("nan")  # kv head 0
+    k[table[0, 6].long(), 0, 0, 5] = float("nan")  # one token of them: left out
+    k[table[0, 6].long(), 1:, :, 2] = 9e3
+    if zero:
+        q[..., 5] = 0.0
+    limit = hip_backend.key_bounds(k.cuda(), _stale(k).cuda(), table.cuda(), lens.cuda())
+    at = table[0, 3].long()
+    assert limit[at, 0, :, 5].tolist() == [float("inf"), float("-inf")]
+    ref = _choice(hip_backend, q, limit.cpu(), table, lens, count, page)
+    first, second = ref[0][0, 0].tolist(), ref[0][0, 1].tolist()
+    assert int(at) not in first and int(at) in second and int(table[0, 6]) in first
+    # Taken where nothing else is left, the earliest such pages first.
+    everything, _ = hip_backend.select_pages(q.cuda(), limit, table.cuda(), lens.cuda(), 9, page)
+    assert int(at) not in everything[0, 0].tolist()
+    k[table[0, 7].long(), :, 0, 8] = float("nan")
+    limit = hip_backend.key_bounds(k.cuda(), limit, table.cuda(), lens.cuda())
+    everything, _ = hip_backend.select_pages(q.cuda(), limit, table.cuda(), lens.cuda(), 9, page)
+    assert int(at) in everything[0, 0].tolist() and int(table[0, 7]) not in everything[0, 0].tolist()
