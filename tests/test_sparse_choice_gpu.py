@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_sparse_attention_gpu import _attend, _case, _choice, _stale
+from tests.test_sparse_attention_gpu import _attend, _bounds, _case, _choice, _stale
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,14 @@ def test_pages_with_a_channel_without_a_number_come_last(hip_backend, H, G, zero
     limit = hip_backend.key_bounds(k.cuda(), limit, table.cuda(), lens.cuda())
     everything, _ = hip_backend.select_pages(q.cuda(), limit, table.cuda(), lens.cuda(), 9, page)
     assert int(at) in everything[0, 0].tolist() and int(table[0, 7]) not in everything[0, 0].tolist()
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_bounds_of_lengths_and_firsts_outside_the_row(hip_backend, page):
+    """A length far beyond the row ends at the row's end, one below zero is none, and neither is anything left behind
+    a ``first`` beyond the length."""
+    _, k, _, table, _ = _case([4 * page] * 4, 2, 2, 64, page, per_row=4)
+    lens = torch.tensor([1 << 30, -7, 2**31 - 1, 3 * page + 1], dtype=torch.int32)
+    _bounds(hip_backend, k, table, lens)
+    _bounds(hip_backend, k, table, lens, torch.tensor([1 << 30, 0, 3 * page, -(1 << 31)], dtype=torch.int32))
+    _bounds(hip_backend, k, table, lens, torch.tensor([4 * page, 5, 2 * page - 1, 3 * page + 1], dtype=torch.int32))
