@@ -230,6 +230,8 @@ int bt_accept_drafts(void* pages, int64_t plane_stride, int64_t page_stride, int
                      void* stream) {
   if (!pages || !aligned16(pages) || planes < 1 || num_pages < 1 || token_elems < 8 || token_elems % 8) return BT_EINVAL;
   if (!table || !lens || !parents || !tokens || !first || !best || !lens_out || !path_out || !following_out) return BT_EINVAL;
+  for (const int32_t* x : {table, lens, parents, tokens, first, best, (const int32_t*)lens_out, (const int32_t*)path_out, (const int32_t*)following_out})
+    if (!aligned4(x)) return BT_EINVAL;
   if (rows < 1 || pages_per_seq < 1 || drafts < 1 || lens_out == lens || following_out == first) return BT_EINVAL;
   if (path_out == parents || path_out == tokens || path_out == best) return BT_EINVAL;
   if (!bt::page_size_served(page_size) || drafts > bt::kMaxDrafts) return BT_ENOTSUP;
@@ -329,7 +331,7 @@ int bt_select_pages(const void* q, int32_t q_dtype, int64_t q_stride_seq, const 
                     const int32_t* lens, int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
                     int32_t count, int32_t* chosen, int32_t* chosen_lens, void* workspace, int64_t workspace_bytes,
                     void* stream) {
-  if (!chosen || !chosen_lens || chosen_lens == lens || chosen == table || !aligned4(chosen)) return BT_EINVAL;
+  if (!chosen || !chosen_lens || chosen_lens == lens || chosen == table || !aligned4(chosen) || !aligned4(chosen_lens)) return BT_EINVAL;
   bt::SelectParams p{};
   const int rc = select_params(p, q, q_dtype, q_stride_seq, bounds, num_pages, page_size, table, table_stride, pages_per_seq,
                                lens, batch, heads, kv_heads, head_dim, count);
@@ -397,7 +399,7 @@ int bt_attn_prep_drafts(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, 
                         int32_t q_dtype, void* k, void* v, int64_t stride_page, int64_t stride_tok, int64_t stride_head,
                         int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_stride,
                         int32_t table_rows, int32_t pages_per_seq, void* stream) {
-  if (!qkv || !pos || !q_out || !aligned16(qkv) || !aligned16(q_out)) return BT_EINVAL;
+  if (!qkv || !pos || !q_out || !aligned16(qkv) || !aligned16(q_out) || !aligned4(angles)) return BT_EINVAL;
   if (tokens < 1 || heads < 1 || kv_heads < 1 || head_dim < 1 || table_rows < 1) return BT_EINVAL;
   if (!dtype_known(qkv_dtype) || !dtype_known(q_dtype)) return BT_EINVAL;
   const int64_t row = (int64_t)heads * head_dim * (gated ? 2 : 1) + 2 * (int64_t)kv_heads * head_dim;
