@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kBoundWaves * 64) void key_bounds_kernel(BoundsPara
 constexpr int kScoreWaves = 4;
 constexpr int kScoreAhead = 4;  // pages whose bounds are on their way, for each group of lanes
 // Waves of one page for each group of lanes up to which there is no more than one: what a wave does shows where few
-// waves are there to hide it.  kScoreAhead / one, us of the sparse attention: 512 waves (4 rows of 127 pages, H = 32, Hkv = 8,
+// waves are there to hide it.  kScoreAhead / one, us of the sparse attention: 1,024 waves (4 rows of 127 pages, H = 32, Hkv = 8,
 // D = 128) 17.35 / 16.3, 2,052 (one of 2,051, H = 16, Hkv = 2, D = 256) 24.0 / 22.8; 4,096 (32 of 128) 33.0 / 34.4.
 constexpr int64_t kFewScoreWaves = 2560;
 // Waves from which on each takes four times as many pages, to load the queries less often.  One / four times, us:
