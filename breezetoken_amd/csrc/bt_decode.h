@@ -1,4 +1,4 @@
-// Device helpers of the decode kernels (gqa_decode.hip, gqa_paged.hip).
+// Device helpers of the decode kernels (gqa_decode.hip, gqa_paged.hip, gqa_tree.hip, page_select.hip).
 #pragma once
 
 #include "bt_common.h"
@@ -11,6 +11,17 @@ template <int V>
 struct IntConst {
   static constexpr int value = V;
 };
+
+// Tiles of a paged K or V in LDS: the 16-byte slot of a row that holds chunk c is c ^
+// slot_of(row), linear in the row's bits, and without bank conflicts (measured) both for the
+// operand reads of K, whose 16 bytes a lane the LDS serves in groups of lanes 0-3, 12-15,
+// 20-23, 24-27 (and so on), and for the transposed reads of V (8 rows, a pair of chunks).
+template <int D>
+__device__ __forceinline__ constexpr int slot_of(int r) {
+  return D == 64 ? r & 6 : (r & 7) * 2;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Raw buffer resource over [base, base + bytes): loads past the end return 0,
 // so tokens past the valid length need no clamping.

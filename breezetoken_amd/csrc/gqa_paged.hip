@@ -50,15 +50,6 @@ __device__ __forceinline__ float term_sum(float v) {
   return v;
 }
 
-// The 16-byte slot of a tile's row that holds chunk c is c ^ slot_of(row): linear in the
-// row's bits, and without bank conflicts (measured) both for the operand reads of K, whose
-// 16 bytes a lane the LDS serves in groups of lanes 0-3, 12-15, 20-23, 24-27 (and so on),
-// and for the transposed reads of V (8 rows, a pair of chunks).
-template <int D>
-__device__ __forceinline__ constexpr int slot_of(int r) {
-  return D == 64 ? r & 6 : (r & 7) * 2;
-}
-
 __device__ __forceinline__ int bcast(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // 64 sequences' lengths and the batch-wide number of their last tile + 1.

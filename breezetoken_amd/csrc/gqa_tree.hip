@@ -51,18 +51,10 @@ constexpr int kPartTiles = 8;
 constexpr int kFewTiles = 2, kManyTiles = 4;
 constexpr float kLazy = 8.0f;  // log2-domain slack before the reference max moves: probabilities stay below 2^8
 
-// The 16-byte slot of a tile's row that holds chunk c is c ^ slot_of(row), as in gqa_paged.hip.
-template <int D>
-__device__ __forceinline__ constexpr int slot_of(int r) {
-  return D == 64 ? r & 6 : (r & 7) * 2;
-}
-
 // HBM -> LDS copy of 16 bytes per lane (lane l's bytes land at lds + 16 * l).
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned char* lds, uint32_t voff, uint32_t soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BT_LDS void*)lds, 16, (int)voff, (int)soff, 0, 0);
 }
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Waits until results of MFMAs can be read, where a branch lies between (hipcc 7.2 puts too few
 // wait states behind one).

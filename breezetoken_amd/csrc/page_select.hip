@@ -23,8 +23,6 @@ namespace bt {
 
 namespace {
 
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // ---------------------------------------------------------------------- bounds
 constexpr int kBoundWaves = 4;
 constexpr int kBoundGroups = 2048;  // work-groups of a launch at most (1,024 and 8,192: 52.3 and 51.7 us for 52.1)
