@@ -29,7 +29,7 @@
 // The MFMA takes K as it is and the query heads of the group as columns.  Scaled
 // queries and probabilities enter as sums of three bf16 terms, which hold all 24 bits
 // of them, in further columns (and, for 5 to 8 heads, a second MFMA).  Two terms, for 5
-// to 8 heads where the output is rounded to bf16 (2^-8), leave 2^-16 (launch_mode).
+// to 8 heads where the output of all pages is rounded to bf16 (2^-8), leave 2^-16 (launch_mode).
 #include "bt_common.h"
 #include "bt_decode.h"
 #include "bt_kernels.h"
@@ -490,10 +490,15 @@ hipError_t launch_terms(const PagedDecodeParams& p, hipStream_t stream) {
 // of 131,072, D = 256 47.2 / 48.3; 16 of 4,000 28.3 / 29.5; one of 500, D = 128, whole 7.4 /
 // 8.2; 512 of 500, D = 64 11.4 / 11.8.  Up to 4 heads (24 of 2,400, D = 128 42.2 / 42.5; 512
 // of 500, D = 64 22.0 / 22.1) the columns are there.
+// Chosen pages (table_stride_head) always take three: beside the choice ahead of them a
+// third costs little.  335 to 391 of 100,000 results to the other side with two, 51 to 63 with
+// three (50 to 56 in plain f32); us of the whole sparse attention, two / three, 8 heads a kv
+// head, 2,048 tokens kept: 32 of 8,000, D = 128 29.4 / 29.6, D = 256 44.9 / 45.7; one of
+// 131,072, D = 256 26.6 / 27.1.
 template <int GMAX, int D, bool WHOLE>
 hipError_t launch_mode(const PagedDecodeParams& p, hipStream_t stream) {
   if constexpr (GMAX > 4) {
-    if (p.out_bf16) return launch_terms<GMAX, D, 2, WHOLE>(p, stream);
+    if (p.out_bf16 && p.table_stride_head == 0) return launch_terms<GMAX, D, 2, WHOLE>(p, stream);
   }
   return launch_terms<GMAX, D, 3, WHOLE>(p, stream);
 }
