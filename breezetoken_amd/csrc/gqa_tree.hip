@@ -22,12 +22,12 @@
 // a kernel behind this one.
 //
 // Measured, both kernels: 32 sequences of 256 to 32,768 tokens, 5 drafts, H = 8, Hkv = 2,
-// D = 256, f32: 102 us, of which this kernel 92, 4.97 TB/s of cache where a large copy reaches
-// 4.93.  24 of 1,800 to 3,000 tokens, 16 drafts, H = 32, Hkv = 8, D = 128, bf16: 65 and 56 us.
-// One of 32,768, 64 drafts, H = 16, Hkv = 2, D = 256, f32: 95 us, 1.08 PFLOP/s of bf16 products
-// (three for each of the formula's; a library's large product reaches 1.2 here).  One of 301,
-// 8 drafts: 14 us, a chain of loads (arguments, length, table, tiles, parts) and of instructions
-// fetched for the first time.
+// D = 256, f32: 94 us, this kernel 91, 5.0 TB/s of cache where a large copy reaches 4.93 and
+// the decode of one token 6.0.  24 of 1,800 to 3,000 tokens, 16 drafts, H = 32, Hkv = 8, D =
+// 128, bf16: 63 and 55 us.  One of 32,768, 64 drafts, H = 16, Hkv = 2, D = 256, f32: 90 us, 1.16
+// PFLOP/s of bf16 products (three for each of the formula's; a library's large product reaches
+// 1.2 here).  One of 301, 8 drafts: 14 us, a chain of loads (arguments, length, table, tiles,
+// parts) and of instructions fetched for the first time.
 #include "bt_common.h"
 #include "bt_decode.h"
 #include "bt_kernels.h"

@@ -13,7 +13,7 @@
 // Bounds are bound by the one read of K: 241 MB (32 sequences of 256 to 32,768 tokens, pages
 // of 32, Hkv = 2, D = 256) in 51 us, 4.7 TB/s where a large copy reaches 4.9; the newest pages
 // of 128 sequences take 5.0 us, a chain of loads.  Scores read 35 MB of bounds (32 sequences of
-// 8,192 to 32,768 tokens, H = 8) in 13 us, 2.7 TB/s, between the stream and the 64-bit products;
+// 8,192 to 32,768 tokens, H = 8) in 13 to 14 us, 2.4 to 2.7 TB/s, between the stream and the 64-bit products;
 // the choice of 63 of up to 1,023 pages takes 6 us, of one among 2,047 5, a chain of barriers.
 #include "bt_common.h"
 #include "bt_decode.h"
